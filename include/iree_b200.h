@@ -566,6 +566,102 @@ iree_b200_status_t iree_b200_w4a16_host(iree_b200_context_t* context, const iree
  * -1 for invalid params. No counterpart in the reference (its HAL leaves transfers to the program). */
 int32_t iree_b200_w4a16_host_plan(const iree_b200_w4a16_params_t* params, int32_t* out_units, int32_t capacity);
 
+/* ---- 4-bit matrix-vector products and the expert layer --------------------------------------------------------------
+ * The dequantisation generic with a zero-point operand (the arith.subf of
+ * compiler/src/iree/compiler/Dialect/Flow/Transforms/test/pipeline_tests.mlir:53-78) and bf16 types, for few rows, and the
+ * mixture-of-experts form of the same product: tokens are sorted by expert, multiplied there, and brought back.
+ *
+ *   w[n, k] = (q[n, k] - zeros[n, k / group]) * scales[n, k / group]   zeros given: q = 0..15
+ *   w[n, k] = q[n, k] * scales[n, k / group]                           zeros NULL: q is two's complement, -8..7
+ *
+ * wq is [N, K/2] bytes (element 2i in the low nibble of byte i, as for iree_b200_w4a16), scales and zeros are [N, K/group]
+ * in the kind's type. Sums are f32 and the result is rounded once; a product whose rows all are finite does not depend on
+ * what other rows or the memory behind the last row hold. Every call queues work on the context's stream and returns; it may
+ * be recorded into a graph (begin_graph); calls share no scratch but the workspace they are given. All pointers are device
+ * pointers: wq on a 16-byte, scales / zeros / activations / results on a 2-byte, index and f32 arrays on a 4-byte boundary
+ * (INVALID_ARGUMENT otherwise). Activations, rows and results on 16-byte boundaries with pitches of whole 16-byte pieces
+ * take the fast paths; others are right and slower. */
+typedef struct {
+  int32_t kind;       /* IREE_B200_KIND_F16 or IREE_B200_KIND_BF16: activations, scales, zeros, result */
+  int32_t M, N, K;    /* 0 <= M <= IREE_B200_MATVEC_MAX_ROWS */
+  int32_t group_size; /* a multiple of 32 that divides K */
+  int32_t lda, ldo;   /* row pitches of a and out, in elements */
+} iree_b200_w4a16_matvec_params_t;
+#define IREE_B200_MATVEC_MAX_ROWS 16
+/* out[M, N] = a[M, K] x w[N, K]^T, the weights read once. Needs no workspace. Under
+ * iree_b200_context_set_dispatch_overlap the weights, scales and zeros are fetched before the dispatch ahead has finished, as
+ * by the decode exports. */
+iree_b200_status_t iree_b200_w4a16_matvec(iree_b200_context_t* context, const iree_b200_w4a16_matvec_params_t* params,
+                                          const void* a, const void* wq, const void* scales, const void* zeros, void* out);
+
+/* Rows of tokens sorted by expert and back. Tables: expert_ids, position and weights are [tokens, slots]; `rows` has
+ * tokens * slots rows, of which offsets[experts] are used. */
+typedef struct {
+  int32_t kind;         /* IREE_B200_KIND_F16 or IREE_B200_KIND_BF16 */
+  int32_t tokens;       /* tokens * slots < 2^31 */
+  int32_t slots;        /* experts per token, 1..256 */
+  int32_t experts;      /* experts of this rank, 1..1024 */
+  int32_t first_expert; /* id of its first one; a slot with an id outside [first_expert, first_expert + experts) is dropped */
+  int32_t width;        /* elements per row */
+  int32_t token_pitch;  /* row pitch of x / out / dout / dx, in elements */
+  int32_t row_pitch;    /* row pitch of rows / drows, in elements */
+} iree_b200_expert_rows_params_t;
+/* Sorts the slots by expert, stable in (token, slot), and copies the tokens' rows there:
+ *   offsets[experts + 1]      rows of the experts before each one; offsets[experts] = rows in all
+ *   position[tokens, slots]   the slot's row, -1 for a dropped slot
+ *   order[tokens * slots]     token * slots + slot of each row, -1 behind the last row
+ *   rows[position[t, j]]      = x[t]; rows behind the last one are left as they were
+ * An id may occur twice in one token: both slots get a row. `workspace` has
+ * iree_b200_expert_dispatch_workspace_bytes(params) bytes (0: NULL will do), 4-byte aligned, need not be initialised and
+ * holds nothing after the call. */
+size_t iree_b200_expert_dispatch_workspace_bytes(const iree_b200_expert_rows_params_t* params);
+iree_b200_status_t iree_b200_expert_dispatch(iree_b200_context_t* context, const iree_b200_expert_rows_params_t* params,
+                                             const int32_t* expert_ids, const void* x, int32_t* offsets, int32_t* position,
+                                             int32_t* order, void* rows, void* workspace);
+/* Its gradient: dx[t] = sum over the token's slots of drows[position[t, j]] (a token whose slots were all dropped: zeros). */
+iree_b200_status_t iree_b200_expert_dispatch_backward(iree_b200_context_t* context,
+                                                      const iree_b200_expert_rows_params_t* params, const void* drows,
+                                                      const int32_t* position, void* dx);
+/* out[t] = sum over the token's slots of weights[t, j] * rows[position[t, j]]; weights are f32. A dropped slot adds nothing,
+ * whatever its weight is. out may not overlap rows. */
+iree_b200_status_t iree_b200_expert_combine(iree_b200_context_t* context, const iree_b200_expert_rows_params_t* params,
+                                            const void* rows, const float* weights, const int32_t* position, void* out);
+/* Its gradients: drows[position[t, j]] = weights[t, j] * dout[t] (rows behind the last one are left as they were),
+ * dweights[t, j] = <dout[t], rows[position[t, j]]> (0 for a dropped slot). drows may not overlap rows. */
+iree_b200_status_t iree_b200_expert_combine_backward(iree_b200_context_t* context,
+                                                     const iree_b200_expert_rows_params_t* params, const void* dout,
+                                                     const void* rows, const float* weights, const int32_t* position,
+                                                     void* drows, float* dweights);
+
+/* The experts' products: row i of `a` belongs to expert e for offsets[e] <= i < offsets[e + 1] and
+ * out[i, n] = sum_k a[i, k] * w[e, n, k], with wq [experts, N, K/2], scales / zeros [experts, N, K/group]. offsets is a
+ * device array as iree_b200_expert_dispatch writes it (read when the dispatch runs); rows of `out` from offsets[experts] on
+ * are left as they were. Variants: STREAM reads each expert's weights for 8 or 16 rows at a time. */
+enum {
+  IREE_B200_W4A16_EXPERTS_AUTO = 0,
+  IREE_B200_W4A16_EXPERTS_STREAM = 1,
+};
+typedef struct {
+  int32_t kind;
+  int32_t experts; /* 1..1024 */
+  int32_t rows;    /* rows of a and out (capacity) */
+  int32_t N, K, group_size;
+  int32_t lda, ldo;
+  int32_t variant; /* IREE_B200_W4A16_EXPERTS_* */
+} iree_b200_w4a16_experts_params_t;
+/* prepare() picks the variant and writes what it needs into the workspace (128-byte aligned, the given size, not shared
+ * between dispatches in flight); run() dispatches and may be repeated while operands stay in place. */
+size_t iree_b200_w4a16_experts_workspace_bytes(const iree_b200_w4a16_experts_params_t* params);
+iree_b200_status_t iree_b200_w4a16_experts_prepare(iree_b200_context_t* context,
+                                                   const iree_b200_w4a16_experts_params_t* params, const void* a,
+                                                   const void* wq, const void* out, void* workspace, int32_t* out_variant);
+iree_b200_status_t iree_b200_w4a16_experts_run(iree_b200_context_t* context, const iree_b200_w4a16_experts_params_t* params,
+                                               const void* a, const void* wq, const void* scales, const void* zeros,
+                                               const int32_t* offsets, void* out, void* workspace, int32_t variant);
+iree_b200_status_t iree_b200_w4a16_experts(iree_b200_context_t* context, const iree_b200_w4a16_experts_params_t* params,
+                                           const void* a, const void* wq, const void* scales, const void* zeros,
+                                           const int32_t* offsets, void* out, void* workspace);
+
 /* ---- sequences of dispatches ----------------------------------------------------------------------
  * `count` dispatches over rotating operand sets issued by one call, i.e. what the reference does
  * when a queue action replays a command buffer that holds that many dispatches

@@ -1762,6 +1762,15 @@ constexpr int kWtMaxDestinations = 8;
 // staging region of the pack / unpack kernels: 64 rows of at most 512 bytes, 16 bytes of padding per row
 constexpr uint32_t kTilingStageBytes = 64 * (2 * 256 + 16);
 
+// b200_w4a16_stream_*: two activation slices, 16 warps x 5 units of 1 KiB, tables
+constexpr uint32_t kStreamSmemBytes = 2 * 66 * 1024 + 16 * 5 * 1024 + 64 * 32 + 1025 * 4 + 256;
+// b200_expert_route: per expert a next row, an offset and 16 warps' counts, and the rows of 512 slots
+constexpr uint32_t kRouteSmemBytes = 4 * (18 * 1024 + 1 + 512);
+constexpr int kMaxExperts = 1024;
+constexpr int kMaxSlots = 256;
+// Up to this many slots every CTA of the routing kernel counts all of them itself (one launch).
+constexpr int64_t kRouteSingleSlots = 8192;
+
 struct EntryDecl {
   const char* name;
   uint32_t block[3];
@@ -1798,6 +1807,16 @@ const EntryDecl kEntries[] = {
     {"b200_w4a16_gemm_wt", {512, 1, 1}, kW4WtSmemBytes},
     {"b200_wait_arrivals", {32, 1, 1}, 0},
     {"b200_w4a16_generic", {256, 1, 1}, 0},
+    {"b200_w4a16_stream_f16_r8", {512, 1, 1}, kStreamSmemBytes},
+    {"b200_w4a16_stream_f16_r16", {512, 1, 1}, kStreamSmemBytes},
+    {"b200_w4a16_stream_bf16_r8", {512, 1, 1}, kStreamSmemBytes},
+    {"b200_w4a16_stream_bf16_r16", {512, 1, 1}, kStreamSmemBytes},
+    {"b200_expert_count", {512, 1, 1}, 0},
+    {"b200_expert_route", {512, 1, 1}, kRouteSmemBytes},
+    {"b200_expert_combine_f16", {256, 1, 1}, 0},
+    {"b200_expert_combine_bf16", {256, 1, 1}, 0},
+    {"b200_expert_combine_backward_f16", {256, 1, 1}, 0},
+    {"b200_expert_combine_backward_bf16", {256, 1, 1}, 0},
     {"b200_mmt4d_s8s8s32", {512, 1, 1}, kMmt4dSmemBytes},
     {"b200_mmt4d_f16f16f32", {512, 1, 1}, kMmt4dSmemBytes},
     {"b200_mmt4d_f16f16f16", {512, 1, 1}, kMmt4dSmemBytes},
@@ -2437,6 +2456,257 @@ iree_b200_status_t iree_b200_matmul_host(iree_b200_context_t* context, const ire
     if (status[0]) return fail(IREE_B200_STATUS_DEADLINE_EXCEEDED, "kernel wait %u ran out at iteration %u", status[0], status[1]);
   }
   return IREE_B200_STATUS_OK;
+}
+
+}  // extern "C"
+
+// ---- 4-bit matrix-vector products and the expert layer ------------------------------------------------------------------
+extern "C" {
+
+static bool misaligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) != 0; }
+
+// One dispatch of the export `name`, which orders itself on the device.
+static iree_b200_status_t dispatch_named(iree_b200_context_t* context, const char* name, int binding_count,
+                                         const void* const* pointers, int constant_count, const int32_t* constants,
+                                         uint32_t grid_x, uint32_t grid_y = 1) {
+  const int32_t ord = iree_hal_b200_executable_lookup(context->executable, name);
+  if (ord < 0) return fail(IREE_B200_STATUS_NOT_FOUND, "export %s missing from the executable", name);
+  auto* cb = context->command_buffer;
+  iree_hal_b200_descriptor_set_binding_t bindings[IREE_HAL_B200_MAX_DESCRIPTOR_SET_BINDING_COUNT];
+  for (int i = 0; i < binding_count; ++i) bindings[i] = {static_cast<uint32_t>(i), const_cast<void*>(pointers[i])};
+  B200_RETURN_IF_ERROR(iree_hal_b200_command_buffer_push_descriptor_set(cb, 0, binding_count, bindings));
+  B200_RETURN_IF_ERROR(iree_hal_b200_command_buffer_push_constants(cb, 0, constants, constant_count * sizeof(int32_t)));
+  return dispatch_self_ordering(context, ord, binding_count, constant_count, grid_x, grid_y);
+}
+
+static iree_b200_status_t stream_validate(int32_t kind, int64_t M, int32_t N, int32_t K, int32_t group, int32_t lda,
+                                          int32_t ldo) {
+  if (kind != IREE_B200_KIND_F16 && kind != IREE_B200_KIND_BF16)
+    return fail(IREE_B200_STATUS_UNIMPLEMENTED, "4-bit weights take f16 or bf16 activations, not kind %d", kind);
+  if (M < 0 || N < 0) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "negative dimension");
+  if (group <= 0 || group % 32 || K <= 0 || K % group)
+    return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "K (%d) must be a positive multiple of a group size (%d) that is a multiple of 32",
+                K, group);
+  if (lda < K || ldo < N)
+    return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "row pitches %d and %d cannot hold %d and %d elements", lda, ldo, K, N);
+  return IREE_B200_STATUS_OK;
+}
+static iree_b200_status_t stream_check_pointers(const void* a, const void* wq, const void* scales, const void* zeros,
+                                                const void* out) {
+  if (!a || !wq || !scales || !out) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "operand pointer is NULL");
+  if (misaligned(wq, 16)) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "weights must start on a 16-byte boundary");
+  if (misaligned(a, 2) || misaligned(scales, 2) || misaligned(zeros, 2) || misaligned(out, 2))
+    return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "activations, scales, zeros and result must start on 2-byte boundaries");
+  return IREE_B200_STATUS_OK;
+}
+// One CTA per SM; a CTA takes an equal part of the weight rows of all passes.
+static iree_b200_status_t stream_dispatch(iree_b200_context_t* context, int32_t kind, bool wide, const void* a,
+                                          const void* wq, const void* scales, const void* zeros, const int32_t* offsets,
+                                          void* out, int32_t M, int32_t N, int32_t K, int32_t group, int32_t lda, int32_t ldo,
+                                          int32_t experts) {
+  const char* name = kind == IREE_B200_KIND_F16 ? (wide ? "b200_w4a16_stream_f16_r16" : "b200_w4a16_stream_f16_r8")
+                                                : (wide ? "b200_w4a16_stream_bf16_r16" : "b200_w4a16_stream_bf16_r8");
+  const void* pointers[6] = {a, wq, scales, zeros, offsets, out};
+  const int32_t constants[7] = {M, N, K, group, lda, ldo, experts};
+  const int sms = usable_sms(context);
+  const int64_t most = static_cast<int64_t>(M) * N;  // passes <= M
+  return dispatch_named(context, name, 6, pointers, 7, constants, static_cast<uint32_t>(most < sms ? most : sms));
+}
+
+iree_b200_status_t iree_b200_w4a16_matvec(iree_b200_context_t* context, const iree_b200_w4a16_matvec_params_t* params,
+                                          const void* a, const void* wq, const void* scales, const void* zeros, void* out) {
+  if (!params) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "params is NULL");
+  const auto& p = *params;
+  B200_RETURN_IF_ERROR(stream_validate(p.kind, p.M, p.N, p.K, p.group_size, p.lda, p.ldo));
+  if (p.M > IREE_B200_MATVEC_MAX_ROWS)
+    return fail(IREE_B200_STATUS_OUT_OF_RANGE, "a matrix-vector product has at most %d rows (got %d)",
+                IREE_B200_MATVEC_MAX_ROWS, p.M);
+  if (p.M && p.N) B200_RETURN_IF_ERROR(stream_check_pointers(a, wq, scales, zeros, out));
+  if (!context) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "context is NULL");
+  if (!p.M || !p.N) return IREE_B200_STATUS_OK;
+  return stream_dispatch(context, p.kind, p.M > 8, a, wq, scales, zeros, nullptr, out, p.M, p.N, p.K, p.group_size, p.lda,
+                         p.ldo, 1);
+}
+
+static iree_b200_status_t experts_validate(const iree_b200_w4a16_experts_params_t* p) {
+  if (!p) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "params is NULL");
+  B200_RETURN_IF_ERROR(stream_validate(p->kind, p->rows, p->N, p->K, p->group_size, p->lda, p->ldo));
+  if (p->experts < 1 || p->experts > kMaxExperts)
+    return fail(IREE_B200_STATUS_OUT_OF_RANGE, "1 to %d experts (got %d)", kMaxExperts, p->experts);
+  if (p->variant != IREE_B200_W4A16_EXPERTS_AUTO && p->variant != IREE_B200_W4A16_EXPERTS_STREAM)
+    return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "unknown variant %d", p->variant);
+  return IREE_B200_STATUS_OK;
+}
+
+size_t iree_b200_w4a16_experts_workspace_bytes(const iree_b200_w4a16_experts_params_t* params) {
+  (void)params;
+  return IREE_B200_WORKSPACE_BYTES;
+}
+
+iree_b200_status_t iree_b200_w4a16_experts_prepare(iree_b200_context_t* context,
+                                                   const iree_b200_w4a16_experts_params_t* params, const void* a,
+                                                   const void* wq, const void* out, void* workspace, int32_t* out_variant) {
+  B200_RETURN_IF_ERROR(experts_validate(params));
+  if (!context) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "context is NULL");
+  if (out_variant) *out_variant = IREE_B200_W4A16_EXPERTS_STREAM;
+  return IREE_B200_STATUS_OK;
+}
+
+iree_b200_status_t iree_b200_w4a16_experts_run(iree_b200_context_t* context, const iree_b200_w4a16_experts_params_t* params,
+                                               const void* a, const void* wq, const void* scales, const void* zeros,
+                                               const int32_t* offsets, void* out, void* workspace, int32_t variant) {
+  B200_RETURN_IF_ERROR(experts_validate(params));
+  const auto& p = *params;
+  if (p.rows && p.N) {
+    B200_RETURN_IF_ERROR(stream_check_pointers(a, wq, scales, zeros, out));
+    if (!offsets || misaligned(offsets, 4))
+      return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "offsets must be a 4-byte aligned device array");
+  }
+  if (!context) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "context is NULL");
+  if (!p.rows || !p.N) return IREE_B200_STATUS_OK;
+  return stream_dispatch(context, p.kind, p.rows > 4 * p.experts, a, wq, scales, zeros, offsets, out, p.rows, p.N, p.K,
+                         p.group_size, p.lda, p.ldo, p.experts);
+}
+
+iree_b200_status_t iree_b200_w4a16_experts(iree_b200_context_t* context, const iree_b200_w4a16_experts_params_t* params,
+                                           const void* a, const void* wq, const void* scales, const void* zeros,
+                                           const int32_t* offsets, void* out, void* workspace) {
+  int32_t variant = 0;
+  B200_RETURN_IF_ERROR(iree_b200_w4a16_experts_prepare(context, params, a, wq, out, workspace, &variant));
+  return iree_b200_w4a16_experts_run(context, params, a, wq, scales, zeros, offsets, out, workspace, variant);
+}
+
+static iree_b200_status_t rows_validate(const iree_b200_expert_rows_params_t* p) {
+  if (!p) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "params is NULL");
+  if (p->kind != IREE_B200_KIND_F16 && p->kind != IREE_B200_KIND_BF16)
+    return fail(IREE_B200_STATUS_UNIMPLEMENTED, "expert rows are f16 or bf16, not kind %d", p->kind);
+  if (p->tokens < 0 || p->width < 0) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "negative dimension");
+  if (p->slots < 1 || p->slots > kMaxSlots)
+    return fail(IREE_B200_STATUS_OUT_OF_RANGE, "1 to %d slots per token (got %d)", kMaxSlots, p->slots);
+  if (p->experts < 1 || p->experts > kMaxExperts)
+    return fail(IREE_B200_STATUS_OUT_OF_RANGE, "1 to %d experts (got %d)", kMaxExperts, p->experts);
+  if (static_cast<int64_t>(p->tokens) * p->slots > INT32_MAX)
+    return fail(IREE_B200_STATUS_OUT_OF_RANGE, "%d tokens x %d slots do not fit 31 bits", p->tokens, p->slots);
+  if (p->token_pitch < p->width || p->row_pitch < p->width)
+    return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "row pitches %d and %d cannot hold %d elements", p->token_pitch, p->row_pitch,
+                p->width);
+  return IREE_B200_STATUS_OK;
+}
+// Elements moved at a time: what widths, pitches and addresses of all arrays allow.
+static int rows_vector(const iree_b200_expert_rows_params_t* p, const void* token_side, const void* row_side,
+                       const void* row_side2) {
+  for (int v = 8; v >= 4; v /= 2)
+    if (p->width % v == 0 && p->token_pitch % v == 0 && p->row_pitch % v == 0 && !misaligned(token_side, 2 * v) &&
+        !misaligned(row_side, 2 * v) && !misaligned(row_side2, 2 * v))
+      return v;
+  return 1;
+}
+static iree_b200_status_t rows_check(const void* a, const void* b, const void* c, const void* d, const void* e, const void* f) {
+  for (const void* p : {a, b, c})  // elements
+    if (misaligned(p, 2)) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "rows must start on 2-byte boundaries");
+  for (const void* p : {d, e, f})  // tables
+    if (misaligned(p, 4)) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "tables must start on 4-byte boundaries");
+  return IREE_B200_STATUS_OK;
+}
+
+// Runs of tokens (grid x) and column parts (grid y) of the routing kernel: two CTAs per SM over the runs, and
+// where there are few tokens their rows cut into parts.
+static void route_grid(const iree_b200_expert_rows_params_t* p, int sms, int* run, int* runs, int* part_width, int* parts) {
+  const int want = 2 * sms;
+  *run = p->tokens > want ? (p->tokens + want - 1) / want : 1;
+  *runs = p->tokens ? (p->tokens + *run - 1) / *run : 1;
+  int cut = sms / *runs;
+  const int most = (p->width + 255) / 256;
+  if (cut > most) cut = most;
+  if (cut < 1) cut = 1;
+  *part_width = ((p->width + cut - 1) / cut + 63) & ~63;
+  if (*part_width < 64) *part_width = 64;
+  *parts = p->width ? (p->width + *part_width - 1) / *part_width : 1;
+}
+
+size_t iree_b200_expert_dispatch_workspace_bytes(const iree_b200_expert_rows_params_t* params) {
+  if (rows_validate(params) != IREE_B200_STATUS_OK) return 0;
+  if (static_cast<int64_t>(params->tokens) * params->slots <= kRouteSingleSlots) return 0;
+  // one histogram per run; at most 2 x 148 runs on any device this library drives, whatever SMs are reserved
+  return static_cast<size_t>(2 * 148) * params->experts * sizeof(int32_t);
+}
+
+iree_b200_status_t iree_b200_expert_dispatch(iree_b200_context_t* context, const iree_b200_expert_rows_params_t* params,
+                                             const int32_t* expert_ids, const void* x, int32_t* offsets, int32_t* position,
+                                             int32_t* order, void* rows, void* workspace) {
+  B200_RETURN_IF_ERROR(rows_validate(params));
+  const auto& p = *params;
+  if (!offsets || (p.tokens && (!expert_ids || !position || !order || (p.width && (!x || !rows)))))
+    return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "operand pointer is NULL");
+  B200_RETURN_IF_ERROR(rows_check(x, rows, nullptr, expert_ids, offsets, position));
+  B200_RETURN_IF_ERROR(rows_check(nullptr, nullptr, nullptr, order, workspace, nullptr));
+  const bool counted = static_cast<int64_t>(p.tokens) * p.slots > kRouteSingleSlots;
+  if (counted && !workspace) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "workspace is NULL");
+  if (!context) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "context is NULL");
+  int sms = usable_sms(context);
+  if (sms > 148) sms = 148;
+  int run, runs, part_width, parts;
+  route_grid(&p, sms, &run, &runs, &part_width, &parts);
+  if (counted) {
+    const void* pointers[2] = {expert_ids, workspace};
+    const int32_t constants[5] = {p.tokens, p.slots, p.experts, p.first_expert, run};
+    B200_RETURN_IF_ERROR(dispatch_named(context, "b200_expert_count", 2, pointers, 5, constants, runs));
+  }
+  const void* pointers[7] = {expert_ids, counted ? workspace : nullptr, x, offsets, position, order, rows};
+  const int32_t constants[10] = {p.tokens, p.slots, p.experts, p.first_expert, run, p.width, p.token_pitch, p.row_pitch,
+                                 part_width, rows_vector(&p, x, rows, nullptr)};
+  return dispatch_named(context, "b200_expert_route", 7, pointers, 10, constants, runs, parts);
+}
+
+static iree_b200_status_t combine_dispatch(iree_b200_context_t* context, const iree_b200_expert_rows_params_t& p,
+                                           const void* rows, const float* weights, const int32_t* position, void* out) {
+  const bool empty = !p.tokens || !p.width;
+  if (!empty && (!rows || !position || !out)) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "operand pointer is NULL");
+  if (!empty && rows == out) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "the result may not overlap the rows");
+  B200_RETURN_IF_ERROR(rows_check(rows, out, nullptr, weights, position, nullptr));
+  if (!context) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "context is NULL");
+  if (empty) return IREE_B200_STATUS_OK;
+  const int vec = rows_vector(&p, out, rows, nullptr);
+  const int64_t strips = (p.width / vec + 63) / 64;
+  const void* pointers[4] = {rows, weights, position, out};
+  const int32_t constants[7] = {p.tokens, p.slots, p.width, p.row_pitch, p.token_pitch, p.tokens * p.slots, vec};
+  return dispatch_named(context, p.kind == IREE_B200_KIND_F16 ? "b200_expert_combine_f16" : "b200_expert_combine_bf16", 4,
+                        pointers, 7, constants, static_cast<uint32_t>((p.tokens * strips + 7) / 8));
+}
+
+iree_b200_status_t iree_b200_expert_combine(iree_b200_context_t* context, const iree_b200_expert_rows_params_t* params,
+                                            const void* rows, const float* weights, const int32_t* position, void* out) {
+  B200_RETURN_IF_ERROR(rows_validate(params));
+  if (params->tokens && params->width && !weights) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "weights are NULL");
+  return combine_dispatch(context, *params, rows, weights, position, out);
+}
+
+iree_b200_status_t iree_b200_expert_dispatch_backward(iree_b200_context_t* context,
+                                                      const iree_b200_expert_rows_params_t* params, const void* drows,
+                                                      const int32_t* position, void* dx) {
+  B200_RETURN_IF_ERROR(rows_validate(params));
+  return combine_dispatch(context, *params, drows, nullptr, position, dx);
+}
+
+iree_b200_status_t iree_b200_expert_combine_backward(iree_b200_context_t* context,
+                                                     const iree_b200_expert_rows_params_t* params, const void* dout,
+                                                     const void* rows, const float* weights, const int32_t* position,
+                                                     void* drows, float* dweights) {
+  B200_RETURN_IF_ERROR(rows_validate(params));
+  const auto& p = *params;
+  if (p.tokens && (!weights || !position || !dweights || (p.width && (!dout || !rows || !drows))))
+    return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "operand pointer is NULL");
+  if (p.tokens && p.width && (drows == rows || drows == dout))
+    return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "drows may not overlap rows or dout");
+  B200_RETURN_IF_ERROR(rows_check(dout, rows, drows, weights, position, dweights));
+  if (!context) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "context is NULL");
+  if (!p.tokens) return IREE_B200_STATUS_OK;
+  const void* pointers[6] = {dout, rows, weights, position, drows, dweights};
+  const int32_t constants[7] = {p.tokens, p.slots, p.width, p.token_pitch, p.row_pitch, p.tokens * p.slots,
+                                rows_vector(&p, dout, rows, drows)};
+  return dispatch_named(context, p.kind == IREE_B200_KIND_F16 ? "b200_expert_combine_backward_f16" : "b200_expert_combine_backward_bf16",
+                        6, pointers, 7, constants,
+                        static_cast<uint32_t>((static_cast<int64_t>(p.tokens) * p.slots + 7) / 8));
 }
 
 }  // extern "C"

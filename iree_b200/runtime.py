@@ -45,6 +45,23 @@ class W4A16Params(C.Structure):
                 ("ldo", C.c_int32), ("n_offset", C.c_int32), ("variant", C.c_int32), ("tile_n", C.c_int32)]
 
 
+class W4A16MatvecParams(C.Structure):
+    _fields_ = [("kind", C.c_int32), ("M", C.c_int32), ("N", C.c_int32), ("K", C.c_int32), ("group_size", C.c_int32),
+                ("lda", C.c_int32), ("ldo", C.c_int32)]
+
+
+class ExpertRowsParams(C.Structure):
+    _fields_ = [("kind", C.c_int32), ("tokens", C.c_int32), ("slots", C.c_int32), ("experts", C.c_int32),
+                ("first_expert", C.c_int32), ("width", C.c_int32), ("token_pitch", C.c_int32), ("row_pitch", C.c_int32)]
+
+
+class W4A16ExpertsParams(C.Structure):
+    _fields_ = [("kind", C.c_int32), ("experts", C.c_int32), ("rows", C.c_int32), ("N", C.c_int32), ("K", C.c_int32),
+                ("group_size", C.c_int32), ("lda", C.c_int32), ("ldo", C.c_int32), ("variant", C.c_int32)]
+
+
+W4A16_EXPERTS_AUTO, W4A16_EXPERTS_STREAM = 0, 1
+W4A16_MATVEC_MAX_ROWS = 16
 W4A16_AUTO, W4A16_DECODE, W4A16_GEMM, W4A16_GENERIC, W4A16_GEMM_WT, W4A16_DECODE_TC = 0, 1, 2, 3, 4, 5
 
 
@@ -79,6 +96,14 @@ def library():
         lib.iree_hal_b200_command_buffer_launch_count.restype = C.c_uint64
         lib.iree_b200_w4a16_workspace_bytes.restype = C.c_size_t
         lib.iree_b200_uk_mmt4d_workspace_bytes.restype = C.c_size_t
+        # the expert layer's calls are short: declared argument types spare an object per argument
+        vp = C.c_void_p
+        for name, args in (("w4a16_matvec", 7), ("w4a16_experts_run", 9), ("w4a16_experts", 9), ("expert_dispatch", 9),
+                           ("expert_dispatch_backward", 5), ("expert_combine", 6), ("expert_combine_backward", 8)):
+            f = getattr(lib, "iree_b200_" + name)
+            f.argtypes = [vp] * args + ([C.c_int32] if name == "w4a16_experts_run" else [])
+        lib.iree_b200_expert_dispatch_workspace_bytes.restype = C.c_size_t
+        lib.iree_b200_w4a16_experts_workspace_bytes.restype = C.c_size_t
         _lib = lib
     return _lib
 
@@ -104,6 +129,15 @@ def _vp(x) -> C.c_void_p:
     if hasattr(x, "data_ptr"):  # a torch tensor on this device
         return C.c_void_p(x.data_ptr())
     raise TypeError(type(x))
+
+
+def _address(x) -> int:
+    """Device address of a torch tensor, a DeviceBuffer, an int, or None."""
+    if x is None:
+        return 0
+    if hasattr(x, "data_ptr"):
+        return x.data_ptr()
+    return _vp(x).value or 0
 
 
 class DeviceBuffer:
@@ -340,6 +374,57 @@ class Context:
     def w4a16_wait_arrivals(self, own_flags, ws, world: int, epoch: int) -> None:
         check(library().iree_b200_w4a16_wait_arrivals(self.handle, _vp(own_flags), _vp(ws), C.c_int32(world),
                                                       C.c_int32(epoch)))
+
+    # 4-bit matrix-vector products and the expert layer. Arrays: torch tensors on this device, DeviceBuffers or addresses.
+    def w4a16_matvec(self, params: W4A16MatvecParams, a, wq, scales, zeros, out) -> None:
+        """out[M, N] = a[M, K] x w[N, K]^T for up to 16 rows; ``zeros`` None: signed weights."""
+        check(library().iree_b200_w4a16_matvec(self.handle, C.addressof(params), _address(a), _address(wq), _address(scales),
+                                               _address(zeros), _address(out)))
+
+    def w4a16_experts_workspace(self, params: W4A16ExpertsParams) -> DeviceBuffer:
+        nbytes = int(library().iree_b200_w4a16_experts_workspace_bytes(C.byref(params)))
+        return DeviceBuffer(self, nbytes).fill(0)
+
+    def w4a16_experts_prepare(self, params: W4A16ExpertsParams, a, wq, out, ws) -> int:
+        variant = C.c_int32()
+        check(library().iree_b200_w4a16_experts_prepare(self.handle, C.byref(params), _vp(a), _vp(wq), _vp(out), _vp(ws),
+                                                        C.byref(variant)))
+        return variant.value
+
+    def w4a16_experts_run(self, params: W4A16ExpertsParams, a, wq, scales, zeros, offsets, out, ws, variant: int) -> None:
+        check(library().iree_b200_w4a16_experts_run(
+            self.handle, C.addressof(params), _address(a), _address(wq), _address(scales), _address(zeros), _address(offsets),
+            _address(out), _address(ws), variant))
+
+    def w4a16_experts(self, params: W4A16ExpertsParams, a, wq, scales, zeros, offsets, out, ws) -> None:
+        check(library().iree_b200_w4a16_experts(
+            self.handle, C.addressof(params), _address(a), _address(wq), _address(scales), _address(zeros), _address(offsets),
+            _address(out), _address(ws)))
+
+    def expert_dispatch_workspace(self, params: ExpertRowsParams) -> Optional[DeviceBuffer]:
+        """None where the dispatch needs none."""
+        nbytes = int(library().iree_b200_expert_dispatch_workspace_bytes(C.byref(params)))
+        return DeviceBuffer(self, nbytes) if nbytes else None
+
+    def expert_dispatch(self, params: ExpertRowsParams, expert_ids, x, offsets, position, order, rows, ws) -> None:
+        """Sorts (token, slot) pairs by expert and copies the tokens' rows there."""
+        check(library().iree_b200_expert_dispatch(self.handle, C.addressof(params), _address(expert_ids), _address(x),
+                                                  _address(offsets), _address(position), _address(order), _address(rows),
+                                                  _address(ws)))
+
+    def expert_dispatch_backward(self, params: ExpertRowsParams, drows, position, dx) -> None:
+        check(library().iree_b200_expert_dispatch_backward(self.handle, C.addressof(params), _address(drows),
+                                                           _address(position), _address(dx)))
+
+    def expert_combine(self, params: ExpertRowsParams, rows, weights, position, out) -> None:
+        """out[t] = sum of weights[t, j] * rows[position[t, j]]."""
+        check(library().iree_b200_expert_combine(self.handle, C.addressof(params), _address(rows), _address(weights),
+                                                 _address(position), _address(out)))
+
+    def expert_combine_backward(self, params: ExpertRowsParams, dout, rows, weights, position, drows, dweights) -> None:
+        check(library().iree_b200_expert_combine_backward(
+            self.handle, C.addressof(params), _address(dout), _address(rows), _address(weights), _address(position),
+            _address(drows), _address(dweights)))
 
     def w4a16_host(self, params: W4A16Params, a, wq, scales, out) -> None:
         check(library().iree_b200_w4a16_host(self.handle, C.byref(params), _vp(a), _vp(wq), _vp(scales), _vp(out)))
