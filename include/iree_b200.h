@@ -636,10 +636,14 @@ iree_b200_status_t iree_b200_expert_combine_backward(iree_b200_context_t* contex
 /* The experts' products: row i of `a` belongs to expert e for offsets[e] <= i < offsets[e + 1] and
  * out[i, n] = sum_k a[i, k] * w[e, n, k], with wq [experts, N, K/2], scales / zeros [experts, N, K/group]. offsets is a
  * device array as iree_b200_expert_dispatch writes it (read when the dispatch runs); rows of `out` from offsets[experts] on
- * are left as they were. Variants: STREAM reads each expert's weights for 8 or 16 rows at a time. */
+ * are left as they were. */
 enum {
   IREE_B200_W4A16_EXPERTS_AUTO = 0,
-  IREE_B200_W4A16_EXPERTS_STREAM = 1,
+  IREE_B200_W4A16_EXPERTS_STREAM = 1, /* reads an expert's weights for 8 or 16 rows at a time; any alignment; rounds only the
+                                         result */
+  IREE_B200_W4A16_EXPERTS_TENSOR = 2, /* tcgen05 tiles of 128 weight rows x up to 256 rows; a and out on 16-byte boundaries,
+                                         lda and ldo multiples of 8, experts * N < 2^31 (INVALID_ARGUMENT otherwise; AUTO then
+                                         picks STREAM); weights are rounded to the kind's type as well */
 };
 typedef struct {
   int32_t kind;

@@ -1764,6 +1764,8 @@ constexpr uint32_t kTilingStageBytes = 64 * (2 * 256 + 16);
 
 // b200_w4a16_stream_*: two activation slices, 16 warps x 5 units of 1 KiB, tables
 constexpr uint32_t kStreamSmemBytes = 2 * 66 * 1024 + 16 * 5 * 1024 + 64 * 32 + 1025 * 4 + 256;
+// b200_w4a16_experts_*: 4 activation stages of 32 KiB, 6 raw stages of 8 KiB, 2 staging tiles of 16 KiB, barriers, tables
+constexpr uint32_t kExpertsSmemBytes = 1024 + 4 * 32768 + 6 * 8192 + 2 * 16384 + 512 + 2 * 1025 * 4 + 56;
 // b200_expert_route: per expert a next row, an offset and 16 warps' counts, and the rows of 512 slots
 constexpr uint32_t kRouteSmemBytes = 4 * (18 * 1024 + 1 + 512);
 constexpr int kMaxExperts = 1024;
@@ -1811,6 +1813,8 @@ const EntryDecl kEntries[] = {
     {"b200_w4a16_stream_f16_r16", {512, 1, 1}, kStreamSmemBytes},
     {"b200_w4a16_stream_bf16_r8", {512, 1, 1}, kStreamSmemBytes},
     {"b200_w4a16_stream_bf16_r16", {512, 1, 1}, kStreamSmemBytes},
+    {"b200_w4a16_experts_f16", {512, 1, 1}, kExpertsSmemBytes},
+    {"b200_w4a16_experts_bf16", {512, 1, 1}, kExpertsSmemBytes},
     {"b200_expert_count", {512, 1, 1}, 0},
     {"b200_expert_route", {512, 1, 1}, kRouteSmemBytes},
     {"b200_expert_combine_f16", {256, 1, 1}, 0},
@@ -2533,9 +2537,23 @@ static iree_b200_status_t experts_validate(const iree_b200_w4a16_experts_params_
   B200_RETURN_IF_ERROR(stream_validate(p->kind, p->rows, p->N, p->K, p->group_size, p->lda, p->ldo));
   if (p->experts < 1 || p->experts > kMaxExperts)
     return fail(IREE_B200_STATUS_OUT_OF_RANGE, "1 to %d experts (got %d)", kMaxExperts, p->experts);
-  if (p->variant != IREE_B200_W4A16_EXPERTS_AUTO && p->variant != IREE_B200_W4A16_EXPERTS_STREAM)
+  if (p->variant < IREE_B200_W4A16_EXPERTS_AUTO || p->variant > IREE_B200_W4A16_EXPERTS_TENSOR)
     return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "unknown variant %d", p->variant);
   return IREE_B200_STATUS_OK;
+}
+static iree_b200_status_t encode_output_map(const void* device_ptr, uint32_t cols, uint32_t rows, uint64_t pitch_bytes,
+                                            void* out_map);
+// What the tensor-core kernel's TMA copies need.
+static bool experts_tensor_fits(const iree_b200_w4a16_experts_params_t* p, const void* a, const void* wq, const void* out) {
+  return !misaligned(a, 16) && !misaligned(wq, 16) && !misaligned(out, 16) && p->lda % 8 == 0 && p->ldo % 8 == 0 &&
+         static_cast<int64_t>(p->experts) * p->N <= INT32_MAX;
+}
+// Rows per expert from which the tensor-core kernel is the faster one.
+constexpr int64_t kExpertsTensorRows = 16;
+static int experts_variant(const iree_b200_w4a16_experts_params_t* p, const void* a, const void* wq, const void* out) {
+  if (p->variant != IREE_B200_W4A16_EXPERTS_AUTO) return p->variant;
+  return p->rows >= kExpertsTensorRows * p->experts && experts_tensor_fits(p, a, wq, out) ? IREE_B200_W4A16_EXPERTS_TENSOR
+                                                                                           : IREE_B200_W4A16_EXPERTS_STREAM;
 }
 
 size_t iree_b200_w4a16_experts_workspace_bytes(const iree_b200_w4a16_experts_params_t* params) {
@@ -2543,13 +2561,53 @@ size_t iree_b200_w4a16_experts_workspace_bytes(const iree_b200_w4a16_experts_par
   return IREE_B200_WORKSPACE_BYTES;
 }
 
+// Rank-3 [1, rows, cols] tensor with a row pitch of its own, swizzled boxes of 64 rows.
+static iree_b200_status_t encode_pitched_map(CUtensorMapDataType type, const void* base, uint32_t cols, uint32_t rows,
+                                             uint64_t pitch_bytes, void* out_map) {
+  B200_RETURN_IF_ERROR(ensure_cuda());
+  CUtensorMap map;
+  const cuuint64_t dims[3] = {cols, rows, 1};
+  const cuuint64_t strides[2] = {pitch_bytes, pitch_bytes * rows};
+  const cuuint32_t box[3] = {64, 64, 1};
+  const cuuint32_t estrides[3] = {1, 1, 1};
+  CU_RETURN_IF_ERROR(g_cu.cuTensorMapEncodeTiled(&map, type, 3, const_cast<void*>(base), dims, strides, box, estrides,
+                                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                                                 CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE),
+                     "cuTensorMapEncodeTiled(activations)");
+  memcpy(out_map, &map, 128);
+  return IREE_B200_STATUS_OK;
+}
+
 iree_b200_status_t iree_b200_w4a16_experts_prepare(iree_b200_context_t* context,
                                                    const iree_b200_w4a16_experts_params_t* params, const void* a,
                                                    const void* wq, const void* out, void* workspace, int32_t* out_variant) {
   B200_RETURN_IF_ERROR(experts_validate(params));
+  const auto& p = *params;
+  const int variant = experts_variant(params, a, wq, out);
+  const bool tensor = variant == IREE_B200_W4A16_EXPERTS_TENSOR && p.rows && p.N;
+  if (tensor) {
+    if (!a || !wq || !out) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "operand pointer is NULL");
+    if (!experts_tensor_fits(params, a, wq, out))
+      return fail(IREE_B200_STATUS_INVALID_ARGUMENT,
+                  "the tensor-core kernel needs 16-byte aligned operands, pitches that are multiples of 8 and experts * N < 2^31");
+    if (!workspace || misaligned(workspace, 128))
+      return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "workspace must be a 128-byte aligned device buffer");
+  }
   if (!context) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "context is NULL");
-  if (out_variant) *out_variant = IREE_B200_W4A16_EXPERTS_STREAM;
-  return IREE_B200_STATUS_OK;
+  if (out_variant) *out_variant = variant;
+  if (!tensor) return IREE_B200_STATUS_OK;
+  if (context->command_buffer->recording)
+    return fail(IREE_B200_STATUS_FAILED_PRECONDITION, "prepare() writes the workspace: call it before a graph is recorded");
+  // header: maps over activations, weights and result, zeroed status words
+  uint8_t host[IREE_B200_WORKSPACE_BYTES];
+  memset(host, 0, sizeof host);
+  B200_RETURN_IF_ERROR(encode_pitched_map(p.kind == IREE_B200_KIND_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                                                        : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                                          a, p.K, p.rows, static_cast<uint64_t>(p.lda) * 2, host));
+  B200_RETURN_IF_ERROR(encode_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, CU_TENSOR_MAP_SWIZZLE_64B, 64, wq, p.K / 2,
+                                  static_cast<uint32_t>(p.experts) * p.N, 1, 64, 128, host + 128));
+  B200_RETURN_IF_ERROR(encode_output_map(out, p.N, p.rows, static_cast<uint64_t>(p.ldo) * 2, host + 256));
+  return iree_hal_b200_transfer_h2d(context->device, host, workspace, sizeof host);
 }
 
 iree_b200_status_t iree_b200_w4a16_experts_run(iree_b200_context_t* context, const iree_b200_w4a16_experts_params_t* params,
@@ -2557,15 +2615,32 @@ iree_b200_status_t iree_b200_w4a16_experts_run(iree_b200_context_t* context, con
                                                const int32_t* offsets, void* out, void* workspace, int32_t variant) {
   B200_RETURN_IF_ERROR(experts_validate(params));
   const auto& p = *params;
+  if (variant != IREE_B200_W4A16_EXPERTS_STREAM && variant != IREE_B200_W4A16_EXPERTS_TENSOR)
+    return fail(IREE_B200_STATUS_FAILED_PRECONDITION, "run() needs the variant that prepare() returned (got %d)", variant);
+  const bool tensor = variant == IREE_B200_W4A16_EXPERTS_TENSOR;
   if (p.rows && p.N) {
     B200_RETURN_IF_ERROR(stream_check_pointers(a, wq, scales, zeros, out));
     if (!offsets || misaligned(offsets, 4))
       return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "offsets must be a 4-byte aligned device array");
+    if (tensor && !experts_tensor_fits(params, a, wq, out))
+      return fail(IREE_B200_STATUS_INVALID_ARGUMENT,
+                  "the tensor-core kernel needs 16-byte aligned operands, pitches that are multiples of 8 and experts * N < 2^31");
+    if (tensor && (!workspace || misaligned(workspace, 128)))
+      return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "workspace must be a 128-byte aligned device buffer");
   }
   if (!context) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "context is NULL");
   if (!p.rows || !p.N) return IREE_B200_STATUS_OK;
-  return stream_dispatch(context, p.kind, p.rows > 4 * p.experts, a, wq, scales, zeros, offsets, out, p.rows, p.N, p.K,
-                         p.group_size, p.lda, p.ldo, p.experts);
+  if (!tensor)
+    return stream_dispatch(context, p.kind, p.rows > 4 * p.experts, a, wq, scales, zeros, offsets, out, p.rows, p.N, p.K,
+                           p.group_size, p.lda, p.ldo, p.experts);
+  // at most one part per 256 rows, and one more per expert
+  const int64_t parts = (p.rows + 255) / 256 + (p.rows < p.experts ? p.rows : p.experts);
+  const int64_t tiles = parts * ((p.N + 127) / 128);
+  const int sms = usable_sms(context);
+  const void* pointers[5] = {scales, zeros, offsets, out, workspace};
+  const int32_t constants[6] = {p.rows, p.N, p.K, p.group_size, p.ldo, p.experts};
+  return dispatch_named(context, p.kind == IREE_B200_KIND_F16 ? "b200_w4a16_experts_f16" : "b200_w4a16_experts_bf16", 5,
+                        pointers, 6, constants, static_cast<uint32_t>(tiles < sms ? tiles : sms));
 }
 
 iree_b200_status_t iree_b200_w4a16_experts(iree_b200_context_t* context, const iree_b200_w4a16_experts_params_t* params,

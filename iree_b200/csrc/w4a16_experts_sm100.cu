@@ -1,0 +1,526 @@
+// The experts' products with 4-bit weights where experts have more than a few rows each: tcgen05 with the dequantised weights
+// as the tensor-memory operand.
+//
+//   out[i, n] = round(sum_k a[i, k] w16[e, n, k]),  w16 = round16((q - z) s)   for rows offsets[e] <= i < offsets[e + 1]
+//
+// The one rounding that is not the result's: a weight enters the tensor core as f16 or bf16, off by half a step of its own value
+// (with a fractional zero point q - z is rounded as well). Its error is random from weight to weight: together with the result's
+// rounding it measures sqrt(2) times the result's alone. Scaling group sums in f32 instead would need the accumulator back in
+// registers for every group, four times the tensor time. Sums are f32 in tensor memory.
+//
+// Roles as in b200_w4a16_gemm_wt: warp 0 fetches activation tiles (TMA, 128-byte swizzle, boxes of 64 rows x 64 K), warp 3 raw
+// weight tiles (128 rows x 128 K), warps 8-15 expand weights into tensor memory (a thread owns a weight row = a lane), one
+// thread of warp 1 issues the matrix instructions two K blocks at a time, warps 4-7 bring the transposed accumulator back.
+// What differs: tiles are (expert, 128 weight rows, up to 256 activation rows), listed from the device's row offsets by every
+// CTA itself. An expert's rows are cut into equal parts of a multiple of 16 (260 rows are 2 x 144, not 256 + 16), and the
+// instruction is only as wide as the part. Rows of the next expert that a box brings along fall into accumulator columns
+// that are not read; a piece of 64 result rows that the expert does not fill is stored by the threads, others by TMA.
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <stdint.h>
+
+#include "sm100_ptx.cuh"
+#include "w4a16_decode.cuh"
+
+namespace b200 {
+
+constexpr int kExWRows = 128;
+constexpr int kExARows = 256;
+constexpr int kExActStages = 4;
+constexpr int kExActStageBytes = kExARows * 128;
+constexpr int kExRawStages = 6;
+constexpr int kExRawStageBytes = kExWRows * 64;
+constexpr int kExAStages = 8;
+constexpr int kExPairStages = kExAStages / 2;
+constexpr int kExAStageColumns = 32;
+constexpr int kExOutRows = 64;
+constexpr int kExOutStageBytes = kExOutRows * kExWRows * 2;
+constexpr int kExThreads = 512;
+constexpr int kExMaxExperts = 1024;
+constexpr int kExBarrierBytes = 512;
+constexpr int kExTableBytes = 2 * (kExMaxExperts + 1) * 4 + 56;
+constexpr int kExSmemBytes = 1024 + kExActStages * kExActStageBytes + kExRawStages * kExRawStageBytes + 2 * kExOutStageBytes +
+                             kExBarrierBytes + kExTableBytes;
+static_assert(kExSmemBytes <= 232448, "per-CTA shared memory limit");
+static_assert(kExARows + kExAStages * kExAStageColumns <= 512, "tensor memory columns");
+
+struct alignas(128) ExWorkspace {
+  uint8_t map_a[128];    // 16-bit [rows, K], 128-byte swizzle, box 64 x 64
+  uint8_t map_w[128];    // u8 [experts * N, K/2], 64-byte swizzle, box 64 x 128
+  uint8_t map_out[128];  // 16-bit [rows, N], no swizzle, box 128 x 64
+  uint32_t status[32];
+};
+
+__device__ __forceinline__ void ex_report(ExWorkspace* ws, uint32_t code, uint32_t info) {
+  if (atomicCAS(&ws->status[0], 0u, code) == 0u) ws->status[1] = info;
+}
+
+struct ExTile {
+  int e, n0, row0, rows;  // rows of the tile, at least one
+};
+
+// Walks the tiles of one CTA; every role has its own.
+struct ExWalk {
+  const int* first;  // tiles before each expert
+  const int* row;    // rows before each expert
+  int tiles_n, e;
+  __device__ ExTile at(int t) {
+    while (first[e + 1] <= t) ++e;
+    const int local = t - first[e], count = row[e + 1] - row[e];
+    const int parts = (count + kExARows - 1) / kExARows;
+    const int per = ((count + parts - 1) / parts + 15) & ~15;
+    const int tn = local / parts, tm = local - tn * parts;
+    ExTile x;
+    x.e = e;
+    x.n0 = tn * kExWRows;
+    x.row0 = row[e] + tm * per;
+    x.rows = min(per, count - tm * per);
+    return x;
+  }
+};
+
+template <bool BF16>
+__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (BF16) asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (BF16) asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+
+// Eight weights in memory order as exact small integers, (w0, w1), (w2, w3), ...: stored values 0..15 or two's complement.
+template <bool BF16, bool ZEROS>
+__device__ __forceinline__ void unpack8_exact(uint32_t v, uint32_t (&q)[4]) {
+  if (BF16) {
+    const uint32_t high = v >> 4;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t pair;  // byte j of v in the low half, of v >> 4 in the high half
+      asm("prmt.b32 %0, %1, %2, %3;" : "=r"(pair) : "r"(v), "r"(high), "r"(0x4400u + 0x1111u * j));
+      // 128 + stored value (top bit flipped: + 8 turns two's complement into value + 8)
+      q[j] = sub2<true>(lop3_and_xor(pair, 0x000f000fu, ZEROS ? 0x43004300u : 0x43084308u), ZEROS ? 0x43004300u : 0x43084308u);
+    }
+  } else {
+    const __half2 mul = __halves2half2(__float2half_rn(1.f), __float2half_rn(0.0625f));
+    const __half2 add = ZEROS ? __halves2half2(__float2half_rn(-1024.f), __float2half_rn(-64.f))
+                              : __halves2half2(__float2half_rn(-1032.f), __float2half_rn(-72.f));
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      uint32_t rep;
+      asm("prmt.b32 %0, %1, %1, %2;" : "=r"(rep) : "r"(v), "r"(0x1111u * j));  // byte j in every byte
+      // low half: 1024 + n_lo; high half: 1024 + 16 n_hi (nibbles' top bits flipped when signed)
+      q[j] = as_u32(__hfma2(as_half2(lop3_and_xor(rep, 0x00f0000fu, ZEROS ? 0x64006400u : 0x64806408u)), mul, add));
+    }
+  }
+}
+
+template <bool BF16, bool ZEROS>
+__device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t* __restrict__ zeros,
+                             const int32_t* __restrict__ offsets, uint16_t* __restrict__ out, ExWorkspace* __restrict__ ws,
+                             int rows, int N, int K, int group, int ldo, int experts) {
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
+  const uint32_t raw_base = smem_base + kExActStages * kExActStageBytes;
+  const uint32_t out_base = raw_base + kExRawStages * kExRawStageBytes;
+  const uint32_t bars = out_base + 2 * kExOutStageBytes;
+  uint8_t* bars_gen = smem_gen + (bars - smem_base);
+  int* tile_first = reinterpret_cast<int*>(bars_gen + kExBarrierBytes);
+  int* row_first = tile_first + kExMaxExperts + 1;
+  auto act_early = [&](int i) { return bars + 8u * i; };  // "the first block of a pair is done with activation stage i"
+  auto raw_full = [&](int i) { return bars + 8u * (kExActStages + i); };
+  auto raw_empty = [&](int i) { return bars + 8u * (kExActStages + kExRawStages + i); };
+  auto a_full = [&](int i) { return bars + 8u * (kExActStages + 2 * kExRawStages + i); };
+  auto a_empty = [&](int i) { return bars + 8u * (kExActStages + 2 * kExRawStages + kExPairStages + i); };
+  constexpr int kNumRingBars = kExActStages + 2 * kExRawStages + 2 * kExPairStages;
+  const uint32_t d_full = bars + 8u * kNumRingBars, d_empty = bars + 8u * (kNumRingBars + 1);
+  const uint32_t tmem_slot = bars + 8u * (kNumRingBars + 2);
+  volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(bars_gen + 8 * (kNumRingBars + 2));
+  volatile uint32_t* abort_flag = reinterpret_cast<volatile uint32_t*>(bars_gen + 8 * (kNumRingBars + 2) + 4);
+  static_assert(8 * (kNumRingBars + 3) <= kExBarrierBytes, "barrier area");
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  grid_launch_dependents();
+  const int tiles_n = (N + kExWRows - 1) / kExWRows;
+  const int num_kb = ((K + 127) >> 7) << 1;  // whole pairs of K blocks; TMA fills K behind the end with zeros
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kExActStages; ++i) mbar_init(act_early(i), 1);
+    for (int i = 0; i < kExRawStages; ++i) {
+      mbar_init(raw_full(i), 1);
+      mbar_init(raw_empty(i), 8);
+    }
+    for (int i = 0; i < kExPairStages; ++i) {
+      mbar_init(a_full(i), 9);  // the eight dequant warps + the activation tiles' expect_tx
+      mbar_init(a_empty(i), 1);
+    }
+    mbar_init(d_full, 1);
+    mbar_init(d_empty, 4);
+    *abort_flag = 0;
+    mbar_fence_init();
+  }
+  if (warp == 2) {
+    tmem_alloc(tmem_slot, 512);
+    tmem_relinquish();
+  }
+  grid_dependency_wait();
+  if (warp == 1) {  // the tile list: rows and tiles before each expert
+    int sum = 0;
+    for (int e0 = 0; e0 < experts; e0 += 32) {
+      const int e = e0 + lane;
+      int lo = 0, need = 0;
+      if (e < experts) {
+        lo = min(max(offsets[e], 0), rows);
+        const int hi = min(max(offsets[e + 1], lo), rows);
+        need = (hi - lo + kExARows - 1) / kExARows * tiles_n;
+      }
+      int incl = need;
+#pragma unroll
+      for (int d = 1; d < 32; d <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += v;
+      }
+      if (e < experts) {
+        tile_first[e] = sum + incl - need;
+        row_first[e] = lo;
+      }
+      sum += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    if (lane == 0) {
+      tile_first[experts] = sum;
+      row_first[experts] = min(max(offsets[experts], 0), rows);
+    }
+  }
+  tc_fence_before_sync();
+  __syncthreads();
+  tc_fence_after_sync();
+  const uint32_t tmem_base = *tmem_slot_ptr;
+  const uint32_t tmem_a = tmem_base + kExARows;
+  const int num_tiles = tile_first[experts];
+  ExWalk walk = {tile_first, row_first, tiles_n, 0};
+
+  if (warp == 0) {
+    // -------- TMA producer of the activation tiles ----------------------------------------------------
+    if (lane == 0) {
+      tensormap_fence_acquire(ws->map_a);
+      uint32_t it = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
+        const ExTile x = walk.at(t);
+        const int boxes = (x.rows + 63) >> 6;
+        for (int kb = 0; kb < num_kb; kb += 2, it += 2) {
+          const uint32_t pair = it >> 1, prev = pair - kExActStages / 2;
+          const uint32_t full = a_full(pair % kExPairStages);
+          bool waited = true;
+          if (pair >= kExActStages / 2) {
+            const uint32_t prev_block = it - kExActStages;
+            waited = mbar_wait(act_early(prev_block % kExActStages), (prev_block / kExActStages) & 1, abort_flag);
+          }
+          if (waited) {
+            mbar_arrive_expect_tx(full, 2 * boxes * 64 * 128);
+            const uint32_t dst = smem_base + (it % kExActStages) * kExActStageBytes;
+            for (int b = 0; b < boxes; ++b) tma_load_3d(dst + b * 64 * 128, ws->map_a, full, kb * 64, x.row0 + b * 64, 0);
+            if (pair >= kExActStages / 2) waited = mbar_wait(a_empty(prev % kExPairStages), (prev / kExPairStages) & 1, abort_flag);
+          }
+          if (!waited) {
+            ex_report(ws, kStatusTimeoutEmpty, it);
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          const uint32_t dst = smem_base + ((it + 1) % kExActStages) * kExActStageBytes;
+          for (int b = 0; b < boxes; ++b)
+            tma_load_3d(dst + b * 64 * 128, ws->map_a, full, (kb + 1) * 64, x.row0 + b * 64, 0);
+        }
+      }
+    }
+  } else if (warp == 3) {
+    // -------- TMA producer of the raw weights: 128 K per stage ------------------------------------------
+    if (lane == 0) {
+      tensormap_fence_acquire(ws->map_w);
+      uint32_t raw_it = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
+        const ExTile x = walk.at(t);
+        for (int g = 0; g < (num_kb >> 1); ++g, ++raw_it) {
+          const int rs = raw_it % kExRawStages;
+          if (!mbar_wait(raw_empty(rs), ((raw_it / kExRawStages) & 1) ^ 1, abort_flag)) {
+            ex_report(ws, kStatusTimeoutEmpty, 0x10000u | raw_it);
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          mbar_arrive_expect_tx(raw_full(rs), kExRawStageBytes);
+          tma_load_3d(raw_base + rs * kExRawStageBytes, ws->map_w, raw_full(rs), g * 64, x.e * N + x.n0, 0);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // -------- MMA issuer -----------------------------------------------------------------------------------
+    if (lane == 0) {
+      const uint64_t desc0 = make_smem_desc(smem_base, 16, 1024);
+      constexpr uint32_t kStageUnits = kExActStageBytes >> 4;
+      uint32_t it = 0, local_tile = 0;
+      bool ok = true;
+      for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x, ++local_tile) {
+        const ExTile x = walk.at(t);
+        const uint32_t idesc =
+            make_instr_desc(1u, BF16 ? 1u : 0u, BF16 ? 1u : 0u, 0u, 0u, kExWRows, static_cast<uint32_t>(x.rows + 15) & ~15u);
+        if (!mbar_wait(d_empty, (local_tile & 1) ^ 1, abort_flag)) {
+          ex_report(ws, kStatusTimeoutTmemEmpty, local_tile);
+          *abort_flag = 1;
+          break;
+        }
+        tc_fence_after_sync();
+        for (int kb = 0; kb < num_kb; kb += 2, it += 2) {
+          const uint32_t pair = it >> 1, ps = pair % kExPairStages;
+          if (!mbar_wait(a_full(ps), (pair / kExPairStages) & 1, abort_flag)) {
+            ex_report(ws, kStatusTimeoutDequant, it);
+            *abort_flag = 1;
+            ok = false;
+            break;
+          }
+          tc_fence_after_sync();
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint64_t bd = desc0 + ((it + h) % kExActStages) * kStageUnits;
+            const uint32_t a_t = tmem_a + ((it + h) % kExAStages) * kExAStageColumns;
+            if (kb == 0 && h == 0) mma_f16_ts_first(tmem_base, a_t, bd, idesc);
+            else mma_f16_ts_more(tmem_base, a_t, bd, idesc);
+            mma_f16_ts_more(tmem_base, a_t + 8, bd + 2, idesc);
+            mma_f16_ts_more(tmem_base, a_t + 16, bd + 4, idesc);
+            mma_f16_ts_more(tmem_base, a_t + 24, bd + 6, idesc);
+            if (h == 0) tc_commit(act_early(it % kExActStages));
+          }
+          tc_commit(a_empty(ps));
+        }
+        if (ok) tc_commit(d_full);
+      }
+    }
+  } else if (warp >= 4 && warp < 8) {
+    // -------- epilogue: D[n, i] -> staged [i, n] pieces -> TMA stores, or the threads' own for a part piece ----
+    const int qd = warp & 3, et = threadIdx.x - 128;
+    const bool issuer = et == 0;
+    if (issuer) tensormap_fence_acquire(ws->map_out);
+    uint32_t local_tile = 0, piece_it = 0;
+    for (int t = blockIdx.x; t < num_tiles; t += gridDim.x, ++local_tile) {
+      const ExTile x = walk.at(t);
+      if (!__all_sync(0xffffffffu, mbar_wait(d_full, local_tile & 1, abort_flag))) {
+        if (lane == 0) {
+          ex_report(ws, kStatusTimeoutTmemFull, local_tile);
+          *abort_flag = 1;
+        }
+        break;
+      }
+      tc_fence_after_sync();
+      const int pieces = (x.rows + kExOutRows - 1) / kExOutRows;
+      for (int pc = 0; pc < pieces; ++pc) {
+        uint32_t v0[32], v1[32];
+        const uint32_t taddr = tmem_base + (static_cast<uint32_t>(qd * 32) << 16) + pc * kExOutRows;
+        tmem_ld_32x32(taddr, v0);
+        tmem_ld_32x32(taddr + 32, v1);
+        tc_wait_ld();
+        if (pc == pieces - 1) {  // the accumulator is in registers / already stored: the next tile's MMAs may start
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(d_empty);
+        }
+        const uint32_t stage = out_base + (piece_it & 1) * kExOutStageBytes;
+        if (issuer) bulk_wait_group_read<1>();  // the store issued from this buffer two pieces ago has read it
+        named_barrier_sync(1, 128);
+        const uint32_t dst = stage + (qd * 32 + lane) * 2;
+#pragma unroll
+        for (int j = 0; j < 32; ++j) {
+          uint16_t h0, h1;
+          if (BF16) {
+            h0 = __bfloat16_as_ushort(__float2bfloat16_rn(__uint_as_float(v0[j])));
+            h1 = __bfloat16_as_ushort(__float2bfloat16_rn(__uint_as_float(v1[j])));
+          } else {
+            h0 = __half_as_ushort(__float2half_rn(__uint_as_float(v0[j])));
+            h1 = __half_as_ushort(__float2half_rn(__uint_as_float(v1[j])));
+          }
+          asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + j * (kExWRows * 2)), "h"(h0) : "memory");
+          asm volatile("st.shared.u16 [%0], %1;" ::"r"(dst + (j + 32) * (kExWRows * 2)), "h"(h1) : "memory");
+        }
+        fence_proxy_async_smem();
+        named_barrier_sync(1, 128);
+        const int left = x.rows - pc * kExOutRows, y = x.row0 + pc * kExOutRows;
+        if (left >= kExOutRows) {
+          if (issuer) tma_store_2d(ws->map_out, stage, x.n0, y);
+        } else {
+          for (int i = et; i < left * (kExWRows / 8); i += 128) {
+            const int r = i >> 4, c = (i & 15) * 8, n = x.n0 + c;
+            const uint4 v = lds128(stage + r * (kExWRows * 2) + c * 2);
+            uint16_t* o = out + static_cast<int64_t>(y + r) * ldo + n;
+            if (n + 8 <= N) {
+              *reinterpret_cast<uint4*>(o) = v;
+            } else {
+              const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (n + j < N) o[j] = static_cast<uint16_t>(words[j >> 1] >> ((j & 1) * 16));
+            }
+          }
+        }
+        if (issuer) bulk_commit_group();  // one group per piece, empty for a part piece
+        ++piece_it;
+      }
+    }
+    if (issuer) bulk_wait_group<0>();
+  } else if (warp >= 8) {
+    // -------- dequant: raw int4 (64-byte swizzled rows) -> 32 columns of this thread's TMEM lane --------------
+    const int td = threadIdx.x - 256;
+    const int r = td & 127;   // weight row of the tile = TMEM lane
+    const int grp = td >> 7;  // K blocks grp, grp + 2, ...
+    const int groups = K / group;
+    const bool halves = (group & 63) != 0;  // a 64-wide block may hold two scale groups
+    const bool octets = (groups & 7) == 0 && !(reinterpret_cast<uintptr_t>(scales) & 15) &&
+                        (!ZEROS || !(reinterpret_cast<uintptr_t>(zeros) & 15));
+    const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
+    uint32_t it_base = 0, raw_it_base = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x, it_base += num_kb, raw_it_base += num_kb >> 1) {
+      const ExTile x = walk.at(t);
+      // rows behind the expert's last one are expanded with its scales and never stored
+      const int64_t srow = (static_cast<int64_t>(x.e) * N + min(x.n0 + r, N - 1)) * groups;
+      // Scales of eight groups arrive as one 16-byte load, one load ahead of their use; else one or two at a time, a block ahead.
+      uint4 sc_cur = make_uint4(0, 0, 0, 0), sc_next = sc_cur, zc_cur = sc_cur, zc_next = sc_cur;
+      uint32_t next_s[2] = {0, 0}, next_z[2] = {0, 0};
+      int cur_octet = -1;
+      auto fetch_block = [&](int kb) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (h == 0 || halves) {
+            const int g = min(kb * 64 + 32 * h, K - 32) / group;
+            next_s[h] = scales[srow + g];
+            if (ZEROS) next_z[h] = zeros[srow + g];
+          }
+        }
+      };
+      if (octets) {
+        sc_next = *reinterpret_cast<const uint4*>(scales + srow);
+        if (ZEROS) zc_next = *reinterpret_cast<const uint4*>(zeros + srow);
+      } else {
+        fetch_block(grp);
+      }
+      for (int kb = grp; kb < num_kb; kb += 2) {
+        const uint32_t it = it_base + kb;
+        const uint32_t raw_it = raw_it_base + (kb >> 1);
+        const int rs = raw_it % kExRawStages;
+        if (!__all_sync(0xffffffffu, mbar_wait(raw_full(rs), (raw_it / kExRawStages) & 1, abort_flag))) {
+          if (lane == 0) {
+            ex_report(ws, kStatusTimeoutFull, 0x10000u | raw_it);
+            *abort_flag = 1;
+          }
+          ok = false;
+          break;
+        }
+        uint32_t s2[2], z2[2] = {0, 0};
+        if (octets) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (h == 0 || halves) {
+              const int g = min(kb * 64 + 32 * h, K - 32) / group;
+              if ((g >> 3) != cur_octet) {  // two blocks advance by at most four groups: never past a whole octet
+                sc_cur = sc_next;
+                zc_cur = zc_next;
+                cur_octet = g >> 3;
+                if ((cur_octet + 1) * 8 < groups) {
+                  sc_next = *reinterpret_cast<const uint4*>(scales + srow + (cur_octet + 1) * 8);
+                  if (ZEROS) zc_next = *reinterpret_cast<const uint4*>(zeros + srow + (cur_octet + 1) * 8);
+                }
+              }
+              const uint32_t sw = (g & 4) ? ((g & 2) ? sc_cur.w : sc_cur.z) : ((g & 2) ? sc_cur.y : sc_cur.x);
+              s2[h] = __byte_perm(sw, 0u, (g & 1) ? 0x3232u : 0x1010u);
+              if (ZEROS) {
+                const uint32_t zw = (g & 4) ? ((g & 2) ? zc_cur.w : zc_cur.z) : ((g & 2) ? zc_cur.y : zc_cur.x);
+                z2[h] = __byte_perm(zw, 0u, (g & 1) ? 0x3232u : 0x1010u);
+              }
+            }
+          }
+        } else {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            s2[h] = __byte_perm(next_s[h], 0u, 0x1010u);
+            if (ZEROS) z2[h] = __byte_perm(next_z[h], 0u, 0x1010u);
+          }
+          if (kb + 2 < num_kb) fetch_block(kb + 2);
+        }
+        if (!halves) {
+          s2[1] = s2[0];
+          z2[1] = z2[0];
+        }
+        const uint32_t pair = it >> 1, ps = pair % kExPairStages;
+        if (!__all_sync(0xffffffffu, mbar_wait(a_empty(ps), ((pair / kExPairStages) & 1) ^ 1, abort_flag))) {
+          if (lane == 0) {
+            ex_report(ws, kStatusTimeoutEmpty, 0x20000u | it);
+            *abort_flag = 1;
+          }
+          ok = false;
+          break;
+        }
+        tc_fence_after_sync();
+        const uint32_t raw_row = raw_base + rs * kExRawStageBytes + r * 64;
+        const int sw_raw = (r >> 1) & 3;
+        uint32_t v[32];  // v[16 c + 4 i + j]: weights 32 c + 8 i + 2 j and the next one, one column of the stage
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int chunk = (kb & 1) * 2 + c;  // 16-byte chunk of the 64-byte raw row = 32 weights
+          const uint4 w = lds128(raw_row + ((chunk ^ sw_raw) << 4));
+          const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t q[4];
+            unpack8_exact<BF16, ZEROS>(words[i], q);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              if (ZEROS) q[j] = sub2<BF16>(q[j], z2[c]);
+              v[16 * c + 4 * i + j] = mul2<BF16>(q[j], s2[c]);
+            }
+          }
+        }
+        tmem_st_32x32(tmem_a + lane_base + (it % kExAStages) * kExAStageColumns, v);
+        tc_wait_st();
+        tc_fence_before_sync();
+        __syncwarp();
+        if (lane == 0) {
+          mbar_arrive(a_full(ps));
+          mbar_arrive(raw_empty(rs));
+        }
+      }
+    }
+  }
+
+  tc_fence_before_sync();
+  __syncthreads();
+  if (*abort_flag) {  // copies in flight land before the block's shared memory is given up
+    const uint64_t t0 = global_timer_ns();
+    while (global_timer_ns() - t0 < 200000ull) {
+    }
+  }
+  if (warp == 2) {
+    tc_fence_after_sync();
+    tmem_dealloc(tmem_base, 512);
+  }
+}
+
+}  // namespace b200
+
+// Bindings: scales, zero points (NULL: signed weights), row offsets, result, workspace.
+#define B200_W4A16_EXPERTS(NAME, BF16)                                                                                     \
+  extern "C" __global__ void __launch_bounds__(b200::kExThreads, 1)                                                        \
+      NAME(const uint16_t* scales, const uint16_t* zeros, const int32_t* offsets, uint16_t* out, void* ws, int rows, int N,  \
+           int K, int group, int ldo, int experts) {                                                                       \
+    b200::ExWorkspace* w = reinterpret_cast<b200::ExWorkspace*>(ws);                                                       \
+    if (zeros) b200::experts_body<BF16, true>(scales, zeros, offsets, out, w, rows, N, K, group, ldo, experts);            \
+    else b200::experts_body<BF16, false>(scales, zeros, offsets, out, w, rows, N, K, group, ldo, experts);                 \
+  }
+B200_W4A16_EXPERTS(b200_w4a16_experts_f16, false)
+B200_W4A16_EXPERTS(b200_w4a16_experts_bf16, true)
+#undef B200_W4A16_EXPERTS

@@ -60,7 +60,7 @@ class W4A16ExpertsParams(C.Structure):
                 ("group_size", C.c_int32), ("lda", C.c_int32), ("ldo", C.c_int32), ("variant", C.c_int32)]
 
 
-W4A16_EXPERTS_AUTO, W4A16_EXPERTS_STREAM = 0, 1
+W4A16_EXPERTS_AUTO, W4A16_EXPERTS_STREAM, W4A16_EXPERTS_TENSOR = 0, 1, 2
 W4A16_MATVEC_MAX_ROWS = 16
 W4A16_AUTO, W4A16_DECODE, W4A16_GEMM, W4A16_GENERIC, W4A16_GEMM_WT, W4A16_DECODE_TC = 0, 1, 2, 3, 4, 5
 

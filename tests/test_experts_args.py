@@ -119,3 +119,25 @@ def test_a_large_dispatch_needs_its_workspace(built):
     p = OK_PTR
     assert status("expert_dispatch", big, p, p, p, p, p, p, None) == 3 and "workspace" in message()
     assert library().iree_b200_expert_dispatch_workspace_bytes(C.byref(rows(tokens=8192, slots=1))) == 0
+
+
+def test_experts_tensor_variant(built):
+    """Alignment and pitches of the tensor-core variant, its workspace, and run() without prepare()'s variant."""
+    P = OK_PTR
+    t = ib.W4A16_EXPERTS_TENSOR
+
+    def run(params, a=P, w=P, o=P, ws=P, variant=t):
+        return status("w4a16_experts_run", params, a, w, P, None, P, o, ws, variant)
+
+    assert run(experts()) == 3 and "context" in message()
+    assert run(experts(), variant=0) == 9 and "prepare" in message()
+    assert run(experts(), variant=7) == 9
+    for bad in (dict(a=P + 8), dict(o=P + 8)):
+        assert run(experts(), **bad) == 3 and "16-byte" in message()
+    assert run(experts(lda=129)) == 3 and run(experts(ldo=65)) == 3 and run(experts(E=1024, N=1 << 22, ldo=1 << 22)) == 3
+    for ws in (None, P + 64):
+        assert run(experts(), ws=ws) == 3 and "workspace" in message()
+        out = C.c_int32()
+        assert library().iree_b200_w4a16_experts_prepare(None, C.byref(experts(variant=t)), C.c_void_p(P), C.c_void_p(P),
+                                                         C.c_void_p(P), C.c_void_p(ws), C.byref(out)) == 3
+        assert "workspace" in message()

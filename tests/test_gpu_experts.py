@@ -364,7 +364,14 @@ def run_experts(ctx, kind, counts, rows, weights, group, a_bits, variant=0, pad_
 
 
 def experts_tolerance(a, w, magnitude, exact, kind, variant):
-    return product_tolerance(a, w, magnitude, exact, kind)
+    """TENSOR rounds a weight to the kind's type (half a step of |w|; q - z is exact for whole zero points) and adds K / 16
+    products of 16 in f32, each off by at most 2^-23 of W so far; AUTO may be either."""
+    tol = product_tolerance(a, w, magnitude, exact, kind)
+    if variant == ib.W4A16_EXPERTS_STREAM:
+        return tol
+    W = np.abs(a) @ np.abs(w).T
+    tensor = HALF_STEP[kind] * (np.abs(exact) + 1.01 * W) + 2.0 ** -25 + (a.shape[-1] / 16 + 1) * 2.0 ** -23 * W
+    return tensor if variant == ib.W4A16_EXPERTS_TENSOR else np.maximum(tol, tensor)
 
 
 def check_experts(ctx, kind, counts, N, K, group, zeros, spare=0, variant=0, seed=0, **layout):
@@ -388,20 +395,40 @@ EXPERT_SHAPES = [  # rows per expert, N, K, group
 ]
 
 
+@pytest.mark.parametrize("variant", [ib.W4A16_EXPERTS_STREAM, ib.W4A16_EXPERTS_TENSOR])
 @pytest.mark.parametrize("kind", [F16, BF16])
 @pytest.mark.parametrize("zeros", [False, True])
 @pytest.mark.parametrize("counts, N, K, group", EXPERT_SHAPES)
-def test_experts(ctx, kind, zeros, counts, N, K, group):
-    check_experts(ctx, kind, counts, N, K, group, zeros, spare=3)
+def test_experts(ctx, variant, kind, zeros, counts, N, K, group):
+    pad = -N % 8 if variant == ib.W4A16_EXPERTS_TENSOR else 0     # its result pitch is a multiple of 8
+    check_experts(ctx, kind, counts, N, K, group, zeros, spare=3, variant=variant, pad_out=pad)
 
 
-@pytest.mark.parametrize("layout", [dict(pad_a=8, pad_out=8), dict(pad_a=1), dict(offset=1), dict(pad_out=3)])
-def test_experts_pitches_and_alignments(ctx, layout):
-    check_experts(ctx, BF16, [4, 0, 21], 72, 320, 64, True, spare=2, **layout)
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("counts", [[256], [257], [255, 64, 128], [600, 0, 1], [16, 17, 63, 64, 65, 66], [1025, 31]])
+def test_experts_tensor_tiles(ctx, kind, counts):
+    """Part tiles of every kind: whole and part pieces of 64 rows, parts of 16 and more rows, N that ends inside a tile."""
+    check_experts(ctx, kind, counts, 200, 384, 64, True, variant=ib.W4A16_EXPERTS_TENSOR)
 
 
-def test_experts_without_rows(ctx):
-    check_experts(ctx, F16, [0, 0, 0], 64, 128, 128, False, spare=5)
+@pytest.mark.parametrize("layout", [dict(pad_a=8, pad_out=8), dict(pad_a=1), dict(offset=1), dict(pad_out=3), dict(pad_a=8, offset=8)])
+@pytest.mark.parametrize("counts", [[4, 0, 21], [40, 70, 30]])
+def test_experts_pitches_and_alignments(ctx, layout, counts):
+    check_experts(ctx, BF16, counts, 72, 320, 64, True, spare=2, **layout)
+
+
+@pytest.mark.parametrize("variant", [ib.W4A16_EXPERTS_STREAM, ib.W4A16_EXPERTS_TENSOR])
+def test_experts_without_rows(ctx, variant):
+    check_experts(ctx, F16, [0, 0, 0], 64, 128, 128, False, spare=5, variant=variant)
+
+
+def test_experts_tensor_refuses_what_its_copies_cannot_reach(ctx):
+    rng = np.random.default_rng(3)
+    w = Weights(rng, F16, 2, 24, 64, 32, False)
+    a = to_bits(rng.standard_normal((8, 64)), F16)
+    for layout in (dict(pad_a=1), dict(pad_out=1), dict(offset=4)):
+        with pytest.raises(ib.IreeB200Error, match="INVALID_ARGUMENT"):
+            run_experts(ctx, F16, [4, 4], 8, w, 32, a, variant=ib.W4A16_EXPERTS_TENSOR, **layout)
 
 
 def layer_buffers(ctx, rng, T, k, E, D, H, group, kind):
@@ -411,11 +438,12 @@ def layer_buffers(ctx, rng, T, k, E, D, H, group, kind):
     return x, ids, weights
 
 
-def test_expert_layer_as_one_recorded_graph(ctx):
+@pytest.mark.parametrize("T", [24, 200])
+def test_expert_layer_as_one_recorded_graph(ctx, T):
     """dispatch -> experts (up) -> experts (down) -> combine, recorded once and replayed on new tokens and new routing, early
     launches on and off; against the same layer in 64 bits with the middle rounded as the calls round it."""
     rng = np.random.default_rng(11)
-    kind, T, k, E, D, H, group = BF16, 24, 2, 8, 128, 192, 64
+    kind, k, E, D, H, group = BF16, 2, 8, 128, 192, 64
     P = T * k
     up, down = Weights(rng, kind, E, H, D, group, True), Weights(rng, kind, E, D, H, group, False)
     dup = [upload(ctx, v) for v in (up.wq, up.scales, up.zeros)]
@@ -463,9 +491,9 @@ def test_expert_layer_as_one_recorded_graph(ctx):
                         continue
                     xe = to_f64(x[t], kind)
                     h64 = up.w[e] @ xe
-                    h_tol = product_tolerance(xe[None], up.w[e], up.magnitude[e], h64[None], kind)[0]
+                    h_tol = experts_tolerance(xe[None], up.w[e], up.magnitude[e], h64[None], kind, 0)[0]
                     y64 = down.w[e] @ h64
-                    y_tol = product_tolerance(h64[None], down.w[e], down.magnitude[e], y64[None], kind)[0] * 1.01 + np.abs(down.w[e]) @ h_tol
+                    y_tol = experts_tolerance(h64[None], down.w[e], down.magnitude[e], y64[None], kind, 0)[0] * 1.01 + 1.01 * np.abs(down.w[e]) @ h_tol
                     want[t] += weights[t, j] * y64
                     bound[t] += weights[t, j] * (y_tol + k * 2.0 ** -24 * np.abs(y64))
             bound += HALF_STEP[kind] * (np.abs(want) + bound)
