@@ -584,7 +584,7 @@ int32_t iree_b200_w4a16_host_plan(const iree_b200_w4a16_params_t* params, int32_
 typedef struct {
   int32_t kind;       /* IREE_B200_KIND_F16 or IREE_B200_KIND_BF16: activations, scales, zeros, result */
   int32_t M, N, K;    /* 0 <= M <= IREE_B200_MATVEC_MAX_ROWS */
-  int32_t group_size; /* a multiple of 32 that divides K */
+  int32_t group_size; /* a multiple of 32 that divides K; K <= 2^20 */
   int32_t lda, ldo;   /* row pitches of a and out, in elements */
 } iree_b200_w4a16_matvec_params_t;
 #define IREE_B200_MATVEC_MAX_ROWS 16

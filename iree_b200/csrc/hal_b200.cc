@@ -1770,6 +1770,7 @@ constexpr uint32_t kExpertsSmemBytes = 1024 + 4 * 32768 + 6 * 8192 + 2 * 16384 +
 constexpr uint32_t kRouteSmemBytes = 4 * (18 * 1024 + 1 + 512);
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxSlots = 256;
+constexpr int kMaxStreamK = 1 << 20;  // the kernels divide K / 32 by group / 32 through a 32-bit reciprocal
 // Up to this many slots every CTA of the routing kernel counts all of them itself (one launch).
 constexpr int64_t kRouteSingleSlots = 8192;
 
@@ -2491,6 +2492,7 @@ static iree_b200_status_t stream_validate(int32_t kind, int64_t M, int32_t N, in
   if (group <= 0 || group % 32 || K <= 0 || K % group)
     return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "K (%d) must be a positive multiple of a group size (%d) that is a multiple of 32",
                 K, group);
+  if (K > kMaxStreamK) return fail(IREE_B200_STATUS_OUT_OF_RANGE, "K is at most %d (got %d)", kMaxStreamK, K);
   if (lda < K || ldo < N)
     return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "row pitches %d and %d cannot hold %d and %d elements", lda, ldo, K, N);
   return IREE_B200_STATUS_OK;

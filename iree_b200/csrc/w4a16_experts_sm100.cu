@@ -94,28 +94,36 @@ __device__ __forceinline__ uint32_t mul2(uint32_t a, uint32_t b) {
   return r;
 }
 
-// Eight weights in memory order as exact small integers, (w0, w1), (w2, w3), ...: stored values 0..15 or two's complement.
-template <bool BF16, bool ZEROS>
-__device__ __forceinline__ void unpack8_exact(uint32_t v, uint32_t (&q)[4]) {
+__device__ __forceinline__ uint32_t twice(uint32_t bits) { return __byte_perm(bits, 0u, 0x1010u); }
+
+// What takes the offset of a stored nibble and its zero point away in one operation, exactly, for a whole zero point: the
+// nibbles arrive as 1024 + n and 64 + n (f16: low and high nibble of a byte) or 128 + n (bf16).
+template <bool BF16>
+__device__ __forceinline__ uint32_t offset_of(float z) {
+  if (BF16) return twice(__bfloat16_as_ushort(__float2bfloat16_rn(128.f + z)));
+  return as_u32(__floats2half2_rn(-1024.f - z, -64.f - z));
+}
+
+// Eight weights in memory order, (w0, w1), (w2, w3), ...: (stored nibble) - (offset) as exact small integers. `flip` turns
+// two's complement into value + 8.
+template <bool BF16, bool FLIP>
+__device__ __forceinline__ void unpack8_minus(uint32_t v, uint32_t offset, uint32_t (&q)[4]) {
   if (BF16) {
     const uint32_t high = v >> 4;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       uint32_t pair;  // byte j of v in the low half, of v >> 4 in the high half
       asm("prmt.b32 %0, %1, %2, %3;" : "=r"(pair) : "r"(v), "r"(high), "r"(0x4400u + 0x1111u * j));
-      // 128 + stored value (top bit flipped: + 8 turns two's complement into value + 8)
-      q[j] = sub2<true>(lop3_and_xor(pair, 0x000f000fu, ZEROS ? 0x43004300u : 0x43084308u), ZEROS ? 0x43004300u : 0x43084308u);
+      q[j] = sub2<true>(lop3_and_xor(pair, 0x000f000fu, FLIP ? 0x43084308u : 0x43004300u), offset);
     }
   } else {
     const __half2 mul = __halves2half2(__float2half_rn(1.f), __float2half_rn(0.0625f));
-    const __half2 add = ZEROS ? __halves2half2(__float2half_rn(-1024.f), __float2half_rn(-64.f))
-                              : __halves2half2(__float2half_rn(-1032.f), __float2half_rn(-72.f));
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       uint32_t rep;
       asm("prmt.b32 %0, %1, %1, %2;" : "=r"(rep) : "r"(v), "r"(0x1111u * j));  // byte j in every byte
-      // low half: 1024 + n_lo; high half: 1024 + 16 n_hi (nibbles' top bits flipped when signed)
-      q[j] = as_u32(__hfma2(as_half2(lop3_and_xor(rep, 0x00f0000fu, ZEROS ? 0x64006400u : 0x64806408u)), mul, add));
+      // low half: 1024 + n_lo; high half: 1024 + 16 n_hi
+      q[j] = as_u32(__hfma2(as_half2(lop3_and_xor(rep, 0x00f0000fu, FLIP ? 0x64806408u : 0x64006400u)), mul, as_half2(offset)));
     }
   }
 }
@@ -154,10 +162,10 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
     for (int i = 0; i < kExActStages; ++i) mbar_init(act_early(i), 1);
     for (int i = 0; i < kExRawStages; ++i) {
       mbar_init(raw_full(i), 1);
-      mbar_init(raw_empty(i), 8);
+      mbar_init(raw_empty(i), 4);
     }
     for (int i = 0; i < kExPairStages; ++i) {
-      mbar_init(a_full(i), 9);  // the eight dequant warps + the activation tiles' expect_tx
+      mbar_init(a_full(i), 5);  // the four warps of a dequant group + the activation tiles' expect_tx
       mbar_init(a_empty(i), 1);
     }
     mbar_init(d_full, 1);
@@ -374,92 +382,105 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
     }
     if (issuer) bulk_wait_group<0>();
   } else if (warp >= 8) {
-    // -------- dequant: raw int4 (64-byte swizzled rows) -> 32 columns of this thread's TMEM lane --------------
+    // -------- dequant: raw int4 (64-byte swizzled rows) -> 64 columns of this thread's TMEM lane, a pair of K blocks at a time --
     const int td = threadIdx.x - 256;
     const int r = td & 127;   // weight row of the tile = TMEM lane
-    const int grp = td >> 7;  // K blocks grp, grp + 2, ...
+    const uint32_t grp = td >> 7;  // pairs grp, grp + 2, ... of the CTA's sequence
     const int groups = K / group;
-    const bool halves = (group & 63) != 0;  // a 64-wide block may hold two scale groups
-    const bool octets = (groups & 7) == 0 && !(reinterpret_cast<uintptr_t>(scales) & 15) &&
-                        (!ZEROS || !(reinterpret_cast<uintptr_t>(zeros) & 15));
+    // Scale groups that a pair (128 K) holds: 1, 2 or 4, aligned with it; or any (a group of 96), one per 32 K.
+    const int per_pair = group % 128 == 0 ? 1 : group == 64 ? 2 : 4;
+    const bool direct = group == 32 || group == 64;   // a pair's scales are neighbours in memory
+    const bool vector = direct && groups % per_pair == 0 && !((reinterpret_cast<uintptr_t>(scales) | reinterpret_cast<uintptr_t>(zeros)) &
+                                                             (2 * per_pair - 1));
+    // block of 32 K -> scale group without a division per pair: exact for (K / 32) (group / 32) < 2^32
+    const uint32_t group_blocks = static_cast<uint32_t>(group) >> 5;
+    const uint32_t magic = group_blocks > 1 ? 0xffffffffu / group_blocks + 1u : 0u;
+    const uint32_t last_block = (static_cast<uint32_t>(K) >> 5) - 1u;
     const uint32_t lane_base = static_cast<uint32_t>((warp & 3) * 32) << 16;
-    uint32_t it_base = 0, raw_it_base = 0;
+    const int pairs = num_kb >> 1;
+    const uint32_t sw_raw = (r >> 1) & 3;
+    uint32_t pair_base = 0;
     bool ok = true;
-    for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x, it_base += num_kb, raw_it_base += num_kb >> 1) {
+    for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x, pair_base += pairs) {
       const ExTile x = walk.at(t);
       // rows behind the expert's last one are expanded with its scales and never stored
       const int64_t srow = (static_cast<int64_t>(x.e) * N + min(x.n0 + r, N - 1)) * groups;
-      // Scales of eight groups arrive as one 16-byte load, one load ahead of their use; else one or two at a time, a block ahead.
-      uint4 sc_cur = make_uint4(0, 0, 0, 0), sc_next = sc_cur, zc_cur = sc_cur, zc_next = sc_cur;
-      uint32_t next_s[2] = {0, 0}, next_z[2] = {0, 0};
-      int cur_octet = -1;
-      auto fetch_block = [&](int kb) {
+      const uint16_t* s_row = scales + srow;
+      const uint16_t* z_row = ZEROS ? zeros + srow : nullptr;
+      uint32_t next_s[4] = {0, 0, 0, 0}, next_z[4] = {0, 0, 0, 0};  // the group's next pair: loaded one turn ahead
+      auto fetch = [&](int p) {
+        if (vector) {
+          if (per_pair == 4) {
+            const uint2 s = *reinterpret_cast<const uint2*>(s_row + p * 4);
+            next_s[0] = s.x & 0xffffu;
+            next_s[1] = s.x >> 16;
+            next_s[2] = s.y & 0xffffu;
+            next_s[3] = s.y >> 16;
+            if (ZEROS) {
+              const uint2 z = *reinterpret_cast<const uint2*>(z_row + p * 4);
+              next_z[0] = z.x & 0xffffu;
+              next_z[1] = z.x >> 16;
+              next_z[2] = z.y & 0xffffu;
+              next_z[3] = z.y >> 16;
+            }
+          } else {
+            const uint32_t s = *reinterpret_cast<const uint32_t*>(s_row + p * 2);
+            next_s[0] = next_s[1] = s & 0xffffu;
+            next_s[2] = next_s[3] = s >> 16;
+            if (ZEROS) {
+              const uint32_t z = *reinterpret_cast<const uint32_t*>(z_row + p * 2);
+              next_z[0] = next_z[1] = z & 0xffffu;
+              next_z[2] = next_z[3] = z >> 16;
+            }
+          }
+        } else {
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (h == 0 || halves) {
-            const int g = min(kb * 64 + 32 * h, K - 32) / group;
-            next_s[h] = scales[srow + g];
-            if (ZEROS) next_z[h] = zeros[srow + g];
+          for (int c = 0; c < 4; ++c) {
+            if (c == 0 || per_pair == 4 || (per_pair == 2 && c == 2)) {
+              const uint32_t block = min(static_cast<uint32_t>(p) * 4 + c, last_block);
+              const uint32_t g = group_blocks > 1 ? __umulhi(block, magic) : block;
+              next_s[c] = s_row[g];
+              if (ZEROS) next_z[c] = z_row[g];
+            } else {
+              next_s[c] = next_s[c - 1];
+              next_z[c] = next_z[c - 1];
+            }
           }
         }
       };
-      if (octets) {
-        sc_next = *reinterpret_cast<const uint4*>(scales + srow);
-        if (ZEROS) zc_next = *reinterpret_cast<const uint4*>(zeros + srow);
-      } else {
-        fetch_block(grp);
-      }
-      for (int kb = grp; kb < num_kb; kb += 2) {
-        const uint32_t it = it_base + kb;
-        const uint32_t raw_it = raw_it_base + (kb >> 1);
-        const int rs = raw_it % kExRawStages;
-        if (!__all_sync(0xffffffffu, mbar_wait(raw_full(rs), (raw_it / kExRawStages) & 1, abort_flag))) {
+      int p = (grp - pair_base) & 1;
+      if (p < pairs) fetch(p);
+      for (; p < pairs; p += 2) {
+        const uint32_t pair = pair_base + p, ps = pair % kExPairStages;
+        const int rs = pair % kExRawStages;
+        uint32_t s2[4], off2[4], z2[4];
+        bool whole = true;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          s2[c] = twice(next_s[c]);
+          if (ZEROS) {
+            const float z = BF16 ? __uint_as_float(next_z[c] << 16) : __half2float(__ushort_as_half(static_cast<uint16_t>(next_z[c])));
+            whole = whole && z == rintf(z) && fabsf(z) <= 64.f;
+            off2[c] = offset_of<BF16>(z);
+            z2[c] = twice(next_z[c]);
+          } else {
+            off2[c] = offset_of<BF16>(8.f);
+            z2[c] = 0;
+          }
+        }
+        if (p + 2 < pairs) fetch(p + 2);
+        const bool fast = !ZEROS || __all_sync(0xffffffffu, whole);
+        if (!__all_sync(0xffffffffu, mbar_wait(raw_full(rs), (pair / kExRawStages) & 1, abort_flag))) {
           if (lane == 0) {
-            ex_report(ws, kStatusTimeoutFull, 0x10000u | raw_it);
+            ex_report(ws, kStatusTimeoutFull, 0x10000u | pair);
             *abort_flag = 1;
           }
           ok = false;
           break;
         }
-        uint32_t s2[2], z2[2] = {0, 0};
-        if (octets) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            if (h == 0 || halves) {
-              const int g = min(kb * 64 + 32 * h, K - 32) / group;
-              if ((g >> 3) != cur_octet) {  // two blocks advance by at most four groups: never past a whole octet
-                sc_cur = sc_next;
-                zc_cur = zc_next;
-                cur_octet = g >> 3;
-                if ((cur_octet + 1) * 8 < groups) {
-                  sc_next = *reinterpret_cast<const uint4*>(scales + srow + (cur_octet + 1) * 8);
-                  if (ZEROS) zc_next = *reinterpret_cast<const uint4*>(zeros + srow + (cur_octet + 1) * 8);
-                }
-              }
-              const uint32_t sw = (g & 4) ? ((g & 2) ? sc_cur.w : sc_cur.z) : ((g & 2) ? sc_cur.y : sc_cur.x);
-              s2[h] = __byte_perm(sw, 0u, (g & 1) ? 0x3232u : 0x1010u);
-              if (ZEROS) {
-                const uint32_t zw = (g & 4) ? ((g & 2) ? zc_cur.w : zc_cur.z) : ((g & 2) ? zc_cur.y : zc_cur.x);
-                z2[h] = __byte_perm(zw, 0u, (g & 1) ? 0x3232u : 0x1010u);
-              }
-            }
-          }
-        } else {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            s2[h] = __byte_perm(next_s[h], 0u, 0x1010u);
-            if (ZEROS) z2[h] = __byte_perm(next_z[h], 0u, 0x1010u);
-          }
-          if (kb + 2 < num_kb) fetch_block(kb + 2);
-        }
-        if (!halves) {
-          s2[1] = s2[0];
-          z2[1] = z2[0];
-        }
-        const uint32_t pair = it >> 1, ps = pair % kExPairStages;
         if (!__all_sync(0xffffffffu, mbar_wait(a_empty(ps), ((pair / kExPairStages) & 1) ^ 1, abort_flag))) {
           if (lane == 0) {
-            ex_report(ws, kStatusTimeoutEmpty, 0x20000u | it);
+            ex_report(ws, kStatusTimeoutEmpty, 0x20000u | pair);
             *abort_flag = 1;
           }
           ok = false;
@@ -467,25 +488,35 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
         }
         tc_fence_after_sync();
         const uint32_t raw_row = raw_base + rs * kExRawStageBytes + r * 64;
-        const int sw_raw = (r >> 1) & 3;
-        uint32_t v[32];  // v[16 c + 4 i + j]: weights 32 c + 8 i + 2 j and the next one, one column of the stage
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int chunk = (kb & 1) * 2 + c;  // 16-byte chunk of the 64-byte raw row = 32 weights
-          const uint4 w = lds128(raw_row + ((chunk ^ sw_raw) << 4));
-          const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+        for (int h = 0; h < 2; ++h) {
+          uint32_t v[32];  // v[16 c + 4 i + j]: weights 32 c + 8 i + 2 j and the next one, one column of the stage
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            uint32_t q[4];
-            unpack8_exact<BF16, ZEROS>(words[i], q);
+          for (int c = 0; c < 2; ++c) {
+            const int chunk = h * 2 + c;  // 16-byte chunk of the 64-byte raw row = 32 weights
+            const uint4 w = lds128(raw_row + ((chunk ^ sw_raw) << 4));
+            const uint32_t words[4] = {w.x, w.y, w.z, w.w};
+            if (fast) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              if (ZEROS) q[j] = sub2<BF16>(q[j], z2[c]);
-              v[16 * c + 4 * i + j] = mul2<BF16>(q[j], s2[c]);
+              for (int i = 0; i < 4; ++i) {
+                uint32_t q[4];
+                unpack8_minus<BF16, !ZEROS>(words[i], off2[chunk], q);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[16 * c + 4 * i + j] = mul2<BF16>(q[j], s2[chunk]);
+              }
+            } else {  // a zero point that is no small whole number: taken away in its own, rounding, step
+              const uint32_t plain = offset_of<BF16>(0.f);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                uint32_t q[4];
+                unpack8_minus<BF16, false>(words[i], plain, q);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[16 * c + 4 * i + j] = mul2<BF16>(sub2<BF16>(q[j], z2[chunk]), s2[chunk]);
+              }
             }
           }
+          tmem_st_32x32(tmem_a + lane_base + ((pair * 2 + h) % kExAStages) * kExAStageColumns, v);
         }
-        tmem_st_32x32(tmem_a + lane_base + (it % kExAStages) * kExAStageColumns, v);
         tc_wait_st();
         tc_fence_before_sync();
         __syncwarp();

@@ -34,6 +34,7 @@ def rows(kind=ib.KIND_F16, tokens=4, slots=2, E=4, first=0, width=64, tp=None, r
     (matvec(kind=ib.KIND_I8), 12, "kind"), (matvec(M=-1), 3, "negative"), (matvec(N=-1, ldo=0), 3, "negative"),
     (matvec(K=0, lda=0), 3, "group"), (matvec(K=100), 3, "group"), (matvec(K=96, group=48), 3, "group"), (matvec(group=0), 3, "group"),
     (matvec(group=-32), 3, "group"), (matvec(lda=127), 3, "pitch"), (matvec(ldo=63), 3, "pitch"), (matvec(M=17), 11, "rows"),
+    (matvec(K=(1 << 20) + 32, group=32), 11, "K is"),
 ])
 def test_matvec_parameters(built, params, code, words):
     assert status("w4a16_matvec", params, OK_PTR, OK_PTR, OK_PTR, None, OK_PTR) == code and words in message()
