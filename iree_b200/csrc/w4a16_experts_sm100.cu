@@ -79,6 +79,13 @@ struct ExWalk {
   }
 };
 
+// True in one thread of the warp.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t one;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+  return one != 0;
+}
+
 template <bool BF16>
 __device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
   uint32_t r;
@@ -213,103 +220,135 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
   const int num_tiles = tile_first[experts];
   ExWalk walk = {tile_first, row_first, tiles_n, 0};
 
+  // The single-thread roles: the whole warp walks the loop and one elected thread issues, so that the operands of copies and
+  // matrix instructions are values which the compiler knows to be uniform and need no move each from a thread's registers
+  // (per pair of K blocks the issuing thread alone took 840 cycles otherwise, against 1024 of the tensor pipe; it takes 330).
+  const int tiles = __shfl_sync(0xffffffffu, num_tiles, 0);
   if (warp == 0) {
     // -------- TMA producer of the activation tiles ----------------------------------------------------
-    if (lane == 0) {
-      tensormap_fence_acquire(ws->map_a);
-      uint32_t it = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
-        const ExTile x = walk.at(t);
-        const int boxes = (x.rows + 63) >> 6;
-        for (int kb = 0; kb < num_kb; kb += 2, it += 2) {
-          const uint32_t pair = it >> 1, prev = pair - kExActStages / 2;
-          const uint32_t full = a_full(pair % kExPairStages);
-          bool waited = true;
-          if (pair >= kExActStages / 2) {
-            const uint32_t prev_block = it - kExActStages;
-            waited = mbar_wait(act_early(prev_block % kExActStages), (prev_block / kExActStages) & 1, abort_flag);
+    const bool leader = elect_one();
+    if (leader) tensormap_fence_acquire(ws->map_a);
+    uint32_t it = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const ExTile x = walk.at(t);
+      const int row0 = __shfl_sync(0xffffffffu, x.row0, 0), boxes = __shfl_sync(0xffffffffu, (x.rows + 63) >> 6, 0);
+      const uint32_t bytes = 2 * boxes * 64 * 128;
+      for (int kb = 0; kb < num_kb; kb += 2, it += 2) {
+        const uint32_t pair = it >> 1, prev = pair - kExActStages / 2;
+        const uint32_t full = a_full(pair % kExPairStages);
+        const uint32_t dst0 = smem_base + (it % kExActStages) * kExActStageBytes;
+        const uint32_t dst1 = smem_base + ((it + 1) % kExActStages) * kExActStageBytes;
+        bool waited = true;
+        if (pair >= kExActStages / 2) {
+          const uint32_t prev_block = it - kExActStages;
+          waited = __all_sync(0xffffffffu, mbar_wait(act_early(prev_block % kExActStages), (prev_block / kExActStages) & 1, abort_flag));
+        }
+        if (waited) {
+          if (leader) {
+            mbar_arrive_expect_tx(full, bytes);
+            tma_load_3d(dst0, ws->map_a, full, kb * 64, row0, 0);
+            if (boxes > 1) tma_load_3d(dst0 + 64 * 128, ws->map_a, full, kb * 64, row0 + 64, 0);
+            if (boxes > 2) tma_load_3d(dst0 + 128 * 128, ws->map_a, full, kb * 64, row0 + 128, 0);
+            if (boxes > 3) tma_load_3d(dst0 + 192 * 128, ws->map_a, full, kb * 64, row0 + 192, 0);
           }
-          if (waited) {
-            mbar_arrive_expect_tx(full, 2 * boxes * 64 * 128);
-            const uint32_t dst = smem_base + (it % kExActStages) * kExActStageBytes;
-            for (int b = 0; b < boxes; ++b) tma_load_3d(dst + b * 64 * 128, ws->map_a, full, kb * 64, x.row0 + b * 64, 0);
-            if (pair >= kExActStages / 2) waited = mbar_wait(a_empty(prev % kExPairStages), (prev / kExPairStages) & 1, abort_flag);
-          }
-          if (!waited) {
+          __syncwarp();
+          if (pair >= kExActStages / 2)
+            waited = __all_sync(0xffffffffu, mbar_wait(a_empty(prev % kExPairStages), (prev / kExPairStages) & 1, abort_flag));
+        }
+        if (!waited) {
+          if (leader) {
             ex_report(ws, kStatusTimeoutEmpty, it);
             *abort_flag = 1;
-            ok = false;
-            break;
           }
-          const uint32_t dst = smem_base + ((it + 1) % kExActStages) * kExActStageBytes;
-          for (int b = 0; b < boxes; ++b)
-            tma_load_3d(dst + b * 64 * 128, ws->map_a, full, (kb + 1) * 64, x.row0 + b * 64, 0);
+          ok = false;
+          break;
         }
+        if (leader) {
+          tma_load_3d(dst1, ws->map_a, full, (kb + 1) * 64, row0, 0);
+          if (boxes > 1) tma_load_3d(dst1 + 64 * 128, ws->map_a, full, (kb + 1) * 64, row0 + 64, 0);
+          if (boxes > 2) tma_load_3d(dst1 + 128 * 128, ws->map_a, full, (kb + 1) * 64, row0 + 128, 0);
+          if (boxes > 3) tma_load_3d(dst1 + 192 * 128, ws->map_a, full, (kb + 1) * 64, row0 + 192, 0);
+        }
+        __syncwarp();
       }
     }
   } else if (warp == 3) {
     // -------- TMA producer of the raw weights: 128 K per stage ------------------------------------------
-    if (lane == 0) {
-      tensormap_fence_acquire(ws->map_w);
-      uint32_t raw_it = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x) {
-        const ExTile x = walk.at(t);
-        for (int g = 0; g < (num_kb >> 1); ++g, ++raw_it) {
-          const int rs = raw_it % kExRawStages;
-          if (!mbar_wait(raw_empty(rs), ((raw_it / kExRawStages) & 1) ^ 1, abort_flag)) {
+    const bool leader = elect_one();
+    if (leader) tensormap_fence_acquire(ws->map_w);
+    uint32_t raw_it = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x) {
+      const ExTile x = walk.at(t);
+      const int w_row = __shfl_sync(0xffffffffu, x.e * N + x.n0, 0);
+      for (int g = 0; g < (num_kb >> 1); ++g, ++raw_it) {
+        const uint32_t rs = raw_it % kExRawStages;
+        if (!__all_sync(0xffffffffu, mbar_wait(raw_empty(rs), ((raw_it / kExRawStages) & 1) ^ 1, abort_flag))) {
+          if (leader) {
             ex_report(ws, kStatusTimeoutEmpty, 0x10000u | raw_it);
             *abort_flag = 1;
-            ok = false;
-            break;
           }
-          mbar_arrive_expect_tx(raw_full(rs), kExRawStageBytes);
-          tma_load_3d(raw_base + rs * kExRawStageBytes, ws->map_w, raw_full(rs), g * 64, x.e * N + x.n0, 0);
+          ok = false;
+          break;
         }
+        if (leader) {
+          mbar_arrive_expect_tx(raw_full(rs), kExRawStageBytes);
+          tma_load_3d(raw_base + rs * kExRawStageBytes, ws->map_w, raw_full(rs), g * 64, w_row, 0);
+        }
+        __syncwarp();
       }
     }
   } else if (warp == 1) {
     // -------- MMA issuer -----------------------------------------------------------------------------------
-    if (lane == 0) {
-      const uint64_t desc0 = make_smem_desc(smem_base, 16, 1024);
-      constexpr uint32_t kStageUnits = kExActStageBytes >> 4;
-      uint32_t it = 0, local_tile = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; t < num_tiles && ok; t += gridDim.x, ++local_tile) {
-        const ExTile x = walk.at(t);
-        const uint32_t idesc =
-            make_instr_desc(1u, BF16 ? 1u : 0u, BF16 ? 1u : 0u, 0u, 0u, kExWRows, static_cast<uint32_t>(x.rows + 15) & ~15u);
-        if (!mbar_wait(d_empty, (local_tile & 1) ^ 1, abort_flag)) {
+    const uint64_t desc0 = make_smem_desc(smem_base, 16, 1024);
+    constexpr uint32_t kStageUnits = kExActStageBytes >> 4;
+    const bool leader = elect_one();
+    const uint32_t d_tmem = __shfl_sync(0xffffffffu, tmem_base, 0), a_tmem = d_tmem + kExARows;
+    uint32_t it = 0, local_tile = 0;
+    bool ok = true;
+    for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++local_tile) {
+      const ExTile x = walk.at(t);
+      const uint32_t n = __shfl_sync(0xffffffffu, static_cast<uint32_t>(x.rows + 15) & ~15u, 0);
+      const uint32_t idesc = make_instr_desc(1u, BF16 ? 1u : 0u, BF16 ? 1u : 0u, 0u, 0u, kExWRows, n);
+      if (!__all_sync(0xffffffffu, mbar_wait(d_empty, (local_tile & 1) ^ 1, abort_flag))) {
+        if (leader) {
           ex_report(ws, kStatusTimeoutTmemEmpty, local_tile);
           *abort_flag = 1;
+        }
+        break;
+      }
+      tc_fence_after_sync();
+      for (int kb = 0; kb < num_kb; kb += 2, it += 2) {
+        const uint32_t pair = it >> 1, ps = pair % kExPairStages;
+        if (!__all_sync(0xffffffffu, mbar_wait(a_full(ps), (pair / kExPairStages) & 1, abort_flag))) {
+          if (leader) {
+            ex_report(ws, kStatusTimeoutDequant, it);
+            *abort_flag = 1;
+          }
+          ok = false;
           break;
         }
         tc_fence_after_sync();
-        for (int kb = 0; kb < num_kb; kb += 2, it += 2) {
-          const uint32_t pair = it >> 1, ps = pair % kExPairStages;
-          if (!mbar_wait(a_full(ps), (pair / kExPairStages) & 1, abort_flag)) {
-            ex_report(ws, kStatusTimeoutDequant, it);
-            *abort_flag = 1;
-            ok = false;
-            break;
-          }
-          tc_fence_after_sync();
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const uint64_t bd = desc0 + ((it + h) % kExActStages) * kStageUnits;
-            const uint32_t a_t = tmem_a + ((it + h) % kExAStages) * kExAStageColumns;
-            if (kb == 0 && h == 0) mma_f16_ts_first(tmem_base, a_t, bd, idesc);
-            else mma_f16_ts_more(tmem_base, a_t, bd, idesc);
-            mma_f16_ts_more(tmem_base, a_t + 8, bd + 2, idesc);
-            mma_f16_ts_more(tmem_base, a_t + 16, bd + 4, idesc);
-            mma_f16_ts_more(tmem_base, a_t + 24, bd + 6, idesc);
-            if (h == 0) tc_commit(act_early(it % kExActStages));
-          }
+        const uint64_t b0 = desc0 + (it % kExActStages) * kStageUnits, b1 = desc0 + ((it + 1) % kExActStages) * kStageUnits;
+        const uint32_t a0 = a_tmem + (it % kExAStages) * kExAStageColumns, a1 = a_tmem + ((it + 1) % kExAStages) * kExAStageColumns;
+        if (leader) {
+          if (kb == 0) mma_f16_ts_first(d_tmem, a0, b0, idesc);
+          else mma_f16_ts_more(d_tmem, a0, b0, idesc);
+          mma_f16_ts_more(d_tmem, a0 + 8, b0 + 2, idesc);
+          mma_f16_ts_more(d_tmem, a0 + 16, b0 + 4, idesc);
+          mma_f16_ts_more(d_tmem, a0 + 24, b0 + 6, idesc);
+          tc_commit(act_early(it % kExActStages));
+          mma_f16_ts_more(d_tmem, a1, b1, idesc);
+          mma_f16_ts_more(d_tmem, a1 + 8, b1 + 2, idesc);
+          mma_f16_ts_more(d_tmem, a1 + 16, b1 + 4, idesc);
+          mma_f16_ts_more(d_tmem, a1 + 24, b1 + 6, idesc);
           tc_commit(a_empty(ps));
         }
-        if (ok) tc_commit(d_full);
+        __syncwarp();
       }
+      if (ok && leader) tc_commit(d_full);
+      __syncwarp();
     }
   } else if (warp >= 4 && warp < 8) {
     // -------- epilogue: D[n, i] -> staged [i, n] pieces -> TMA stores, or the threads' own for a part piece ----
