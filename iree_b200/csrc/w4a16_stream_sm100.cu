@@ -11,15 +11,16 @@
 // A nibble becomes a 16-bit float by a shift and one logic operation for two weights: under the exponent of 64 (f16: its bits
 // land in mantissa bits 4..7) or 128 (bf16: bits 0..3), and z' grows by that much; the part that cancels is at most 158 / 15 of
 // the sum it leaves, 2^-20 of it in f32. (f16 subnormals, q 2^-24 as stored, would spare the shifts; but the tensor core
-// aligns products by their exponent fields, and sums lost up to six more bits there.) The sums of a are one more row of ones
-// in the matrix instruction, shared by all weight tiles of a warp.
+// aligns products by their exponent fields, and sums lost up to six more bits there.) The accumulator starts
+// at minus that offset times the sum of a.
 //
 // Work. The weight rows of all active experts (one, for a matrix-vector product) form one list; every CTA gets an equal
 // part of it, to the row, so that all SMs read the same number of bytes (tiles of 16 rows alone would leave the last round
-// half empty: 688 tiles on 148 SMs are 4.65 rounds). A CTA's warps are WK along K x WN along N, chosen by the CTA for the
-// rows it holds; a warp walks units of 16 rows x 128 K through a private ring of cp.async stages (no barrier between
-// warps), and the WK partial sums meet in shared memory at the end, in order: results do not depend on timing.
-// Activations are staged in slices, the next one while the present one is used.
+// half empty: 688 tiles on 148 SMs are 4.65 rounds). A batch is up to 512 rows of the part: its row pairs of tiles (32 rows)
+// go to WN warp columns and K to WK warps of each, WN x WK <= 16. A warp walks units of 32 rows x 128 K through a private
+// ring of cp.async stages (no barrier between warps, and none between batches), and the WK partial sums meet in shared
+// memory, in order: results do not depend on timing. Activations are staged in slices of K, the next slice while the present
+// one is used; staging orders them as the unpacked nibbles come (k, k + 4) and leaves the sums of each scale block beside them.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
@@ -31,13 +32,16 @@ namespace b200 {
 
 constexpr int kStreamThreads = 512;
 constexpr int kStreamWarps = kStreamThreads / 32;
-constexpr int kStreamRing = 5;                        // units in flight per warp (4) and the one in use: 64 KiB per SM in flight
-constexpr int kStreamUnitBytes = 1024;                // 16 weight rows x 128 K
-constexpr int kStreamActBytes = 66 * 1024;            // one activation slice: 8 NB rows x (4096 / NB) K, 64 bytes of padding per row
-constexpr int kStreamBatchMax = 64;                   // batches described at a time
+constexpr int kStreamRing = 3;                        // units per warp: two in flight, 64 KiB per SM, and the one in use
+constexpr int kStreamUnitBytes = 2048;                // 32 weight rows x 128 K
+constexpr int kStreamActBytes = 33 * 1024;            // one activation slice
+constexpr int kStreamSumBytes = 2 * 4096;             // its sums, and the sums times the offset of the unpacked nibbles
+constexpr int kStreamRedBytes = kStreamWarps * 2 * 16 * 20 * 4;  // partial sums of 16 warps x 32 rows x 16 activation rows
+constexpr int kStreamBatchMax = 32;                   // batches described at a time
 constexpr int kStreamMaxExperts = 1024;
-constexpr int kStreamTableBytes = kStreamBatchMax * 32 + (kStreamMaxExperts + 1) * 4 + 256;
-constexpr int kStreamSmemBytes = 2 * kStreamActBytes + kStreamWarps * kStreamRing * kStreamUnitBytes + kStreamTableBytes;
+constexpr int kStreamTableBytes = kStreamBatchMax * 32 + (kStreamMaxExperts + 1) * 4 + 60;
+constexpr int kStreamSmemBytes = kStreamWarps * kStreamRing * kStreamUnitBytes + 2 * (kStreamActBytes + kStreamSumBytes) +
+                                 kStreamRedBytes + kStreamTableBytes;
 static_assert(kStreamSmemBytes <= 232448, "per-CTA shared memory limit");
 
 struct StreamBatch {
@@ -46,8 +50,8 @@ struct StreamBatch {
   int32_t nrows;    // weight rows
   int32_t a_row;    // first activation row
   int32_t mrows;    // activation rows
-  int32_t wk_log2;  // warps along K
-  int32_t pad;
+  int32_t wn;       // warp columns = pairs of tiles
+  int32_t wk;       // warps along K of each
 };
 static_assert(sizeof(StreamBatch) == 32, "table size");
 
@@ -98,33 +102,42 @@ struct StreamArgs {
 // NB: blocks of 8 activation rows a pass covers; GQ: 32-wide K blocks per scale application (group % (32 GQ) == 0).
 template <bool BF16, int NB, int GQ>
 __device__ void stream_body(const StreamArgs& p) {
-  // weight tiles per warp: what fits the registers, and the partial sums of 16 warps one activation buffer
-  constexpr int TM = NB == 1 ? 4 : 3;
-  constexpr int kSliceK = 4096 / NB;
-  constexpr int kActPitch = kSliceK * 2 + 64;      // bytes; 64 mod 128: eight lanes of a 16-byte read hit all banks
   constexpr int kRedPitch = 20;                    // floats per activation row of a partial tile (16 + padding)
-  constexpr int kBlocks = 4 / GQ;                  // scale applications per chunk
-  static_assert(8 * NB * kActPitch <= kStreamActBytes, "activation slice");
-  static_assert(kStreamWarps * TM * 8 * NB * kRedPitch * 4 <= kStreamActBytes, "partial sums");
+  constexpr int kTile = 8 * NB * kRedPitch;
+  constexpr int kBlocks = 4 / GQ;                  // scale blocks per chunk of 128 K
+  constexpr int kCols = 8 * NB;
+  static_assert(kStreamWarps * 2 * kTile * 4 <= kStreamRedBytes, "partial sums");
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t smem = smem_u32(smem_raw);
-  uint8_t* table_gen = smem_raw + 2 * kStreamActBytes + kStreamWarps * kStreamRing * kStreamUnitBytes;
-  StreamBatch* batches = reinterpret_cast<StreamBatch*>(table_gen);
-  int* seg_first = reinterpret_cast<int*>(table_gen + kStreamBatchMax * 32);  // passes before each expert
-  int* shared_words = seg_first + kStreamMaxExperts + 1;                      // [0] batches in the table
+  constexpr int kActOffset = kStreamWarps * kStreamRing * kStreamUnitBytes;
+  constexpr int kSumOffset = kActOffset + 2 * kStreamActBytes;
+  constexpr int kRedOffset = kSumOffset + 2 * kStreamSumBytes;
+  constexpr int kTableOffset = kRedOffset + kStreamRedBytes;
+  StreamBatch* batches = reinterpret_cast<StreamBatch*>(smem_raw + kTableOffset);
+  int* seg_first = reinterpret_cast<int*>(smem_raw + kTableOffset + kStreamBatchMax * 32);  // passes before each expert
+  int* shared_words = seg_first + kStreamMaxExperts + 1;                                    // [0] batches in the table
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-  const uint32_t ring = smem + 2 * kStreamActBytes + warp * (kStreamRing * kStreamUnitBytes);
   const int chunks = (p.K + 127) >> 7;
-  const int slices = (p.K + kSliceK - 1) / kSliceK;
+  // A slice holds the rows of one pass: as much of K as fits the buffers, in whole chunks.
+  const int pass_rows = min(p.M, kCols);
+  const int most_k = min((kStreamActBytes / pass_rows - 64) >> 1, (kStreamSumBytes / 2) / (4 * kCols) * 32 * GQ);
+  const int fewest = (p.K + (most_k & ~127) - 1) / (most_k & ~127);
+  const int slice_chunks = (chunks + fewest - 1) / fewest, slices = (chunks + slice_chunks - 1) / slice_chunks;
+  const int slice_k = slice_chunks << 7;
+  const int act_pitch = slice_k * 2 + 64;          // bytes; 64 mod 128: eight lanes of a 16-byte read hit all banks
   const bool acts_aligned = !((reinterpret_cast<uintptr_t>(p.a) | (static_cast<uintptr_t>(p.lda) * 2)) & 15);
   const int groups = p.K / p.group;
+  // block of 32 K -> scale group without a division: exact for (K / 32) (group / 32) < 2^32
+  const uint32_t group_blocks = static_cast<uint32_t>(p.group) >> 5;
+  const uint32_t magic = group_blocks > 1 ? 0xffffffffu / group_blocks + 1u : 0u;
+  const int last_block = (p.K >> 5) - 1;
   const int64_t w_pitch = p.K >> 1;
 
   grid_launch_dependents();
   // Experts: how many passes (8 NB activation rows each) each one needs comes from the dispatch ahead.
-  int passes = (p.M + 8 * NB - 1) / (8 * NB);
+  int passes = (p.M + kCols - 1) / kCols;
   if (p.offsets) {
     grid_dependency_wait();
     if (warp == 0) {
@@ -134,7 +147,7 @@ __device__ void stream_body(const StreamArgs& p) {
         int need = 0;
         if (e < p.experts) {
           const int lo = min(max(p.offsets[e], 0), p.M), hi = min(max(p.offsets[e + 1], lo), p.M);
-          need = (hi - lo + 8 * NB - 1) / (8 * NB);
+          need = (hi - lo + kCols - 1) / kCols;
         }
         int incl = need;
 #pragma unroll
@@ -157,15 +170,14 @@ __device__ void stream_body(const StreamArgs& p) {
   bool waited = p.offsets != nullptr;
   const uint32_t mask = BF16 ? 0x000f000fu : 0x00f000f0u;
   const uint32_t under = BF16 ? (p.zeros ? 0x43004300u : 0x43084308u) : (p.zeros ? 0x54005400u : 0x54805480u);
-  const uint32_t ones = BF16 ? 0x3f803f80u : 0x3c003c00u;
-  const float z_base = BF16 ? 128.f : 64.f;
+  // what the unpacked nibbles stand above their values: of all of them, or without the zero points
+  const float above = (BF16 ? 128.f : 64.f) + (p.zeros ? 0.f : 8.f);
 
   while (row < row_end) {  // one turn for up to kStreamBatchMax batches: one, unless the operands are very uneven
     __syncthreads();
     if (tid == 0) {
-      int count = 0;
-      int e = 0;
-      int64_t pass = row / p.N;
+      int count = 0, e = 0;
+      int64_t pass = total == p.N ? 0 : row / p.N;
       if (p.offsets) {
         int lo = 0, hi = p.experts;  // last expert whose first pass is <= pass
         while (hi - lo > 1) {
@@ -186,132 +198,145 @@ __device__ void stream_body(const StreamArgs& p) {
           have = min(max(p.offsets[e + 1], first), p.M) - first;
           nth = static_cast<int>(pass) - seg_first[e];
         }
-        // Warps along K: the split with the fewest units for the busiest warp; ties to more warps along K (more
-        // tiles per warp share the activation fragments).
-        const int64_t cap = 8 * TM * 16;
-        const int64_t parts = (left + cap - 1) / cap;
-        const int nrows = static_cast<int>((left + parts - 1) / parts);
-        const int tiles = (nrows + 15) >> 4;
-        int best = 1, best_units = 0x7fffffff;
-        for (int l = 4; l >= 1; --l) {
-          const int wn = kStreamWarps >> l, per = (tiles + wn - 1) / wn;
-          if (per > TM) continue;
-          int units = 0;
-          for (int s = 0; s < slices; ++s) {
-            const int in_slice = min(kSliceK / 128, chunks - s * (kSliceK / 128));
-            units += per * ((in_slice + (1 << l) - 1) >> l);
-          }
-          if (units < best_units) {
-            best_units = units;
-            best = l;
-          }
-        }
+        // Pairs of tiles that leave few of the 16 warps idle: 1-5, 7, 8, 13-16; others are cut at 4 or 8 pairs.
+        int pairs = static_cast<int>(min(left + 31, static_cast<int64_t>(512)) >> 5);
+        if (pairs == 6) pairs = 4;
+        else if (pairs > 8 && pairs < 13) pairs = 8;
         StreamBatch b;
         b.w_row = static_cast<int64_t>(e) * p.N + n0;
         b.n0 = n0;
-        b.nrows = nrows;
-        b.a_row = first + nth * 8 * NB;
-        b.mrows = min(8 * NB, have - nth * 8 * NB);
-        b.wk_log2 = best;
-        b.pad = 0;
+        b.nrows = static_cast<int>(min(left, static_cast<int64_t>(pairs * 32)));
+        b.a_row = first + nth * kCols;
+        b.mrows = min(kCols, have - nth * kCols);
+        b.wn = pairs;
+        b.wk = kStreamWarps / pairs;
         batches[count++] = b;
-        r += nrows;
-        if (n0 + nrows == p.N) ++pass;
+        r += b.nrows;
+        if (n0 + b.nrows == p.N) ++pass;
       }
       shared_words[0] = count;
     }
     __syncthreads();
     const int count = shared_words[0];
-    {
-      int64_t covered = 0;
-      for (int i = 0; i < count; ++i) covered += batches[i].nrows;
-      row += covered;
-    }
+    for (int i = 0; i < count; ++i) row += batches[i].nrows;
     const int steps = count * slices;
 
-    // ---- unit sequence of this warp: (step = batch x slice, chunk of the slice, tile) ---------------------------------
-    int is_step = -1, is_chunk = 0, is_chunks = 0, is_tile = 0, is_tiles = 0, is_slot = 0, is_wk = 0, is_wn = 0;
-    StreamBatch is_b;
-    uint32_t q0 = 0, q1 = 0, q2 = 0, q3 = 0;  // scales (low half) and zeros (high half) of the units in flight, rows g
-    uint32_t r0 = 0, r1 = 0, r2 = 0, r3 = 0;  // rows g + 8
-    auto issue_step = [&]() {  // moves the issue cursor to the next step in which this warp has a unit
-      while (++is_step < steps) {
-        const int b = is_step / slices, s = is_step - b * slices;
-        is_b = batches[b];
-        const int wk_n = 1 << is_b.wk_log2, wn_n = kStreamWarps >> is_b.wk_log2;
-        is_wk = warp & (wk_n - 1);
-        is_wn = warp >> is_b.wk_log2;
-        const int tiles = (is_b.nrows + 15) >> 4;
-        is_tiles = (tiles - is_wn + wn_n - 1) / wn_n;
-        const int first = s * (kSliceK / 128);
-        is_chunk = first + is_wk;
-        is_chunks = min(chunks, first + kSliceK / 128);
-        is_tile = 0;
-        if (is_tiles > 0 && is_chunk < is_chunks) return;
+    // ---- unit sequence of this warp: (batch, chunk = wk, wk + WK, ...), ahead of its use ---------------------------------
+    int is_batch = -1, is_chunk = chunks, is_wk = 0, is_slot = 0;
+    const uint8_t* is_w = nullptr;       // this lane's 16 bytes of row g of the pair, K = 0
+    int32_t is_off1 = 0, is_off2 = 0, is_off3 = 0;  // bytes from there to rows g + 8, g + 16, g + 24 (the last row for rows behind it)
+    int64_t is_s = 0;                    // first scale of row g + 8 t
+    auto issue_batch = [&]() {  // the next batch in which this warp has a unit
+      while (++is_batch < count) {
+        const StreamBatch b = batches[is_batch];
+        const int wk = warp / b.wn, wn = warp - wk * b.wn;
+        if (wk >= b.wk || wk >= chunks) continue;
+        const int r0 = wn * 32, last = b.nrows - 1;
+        const int64_t first = b.w_row + min(r0 + g, last);
+        is_w = p.wq + first * w_pitch;
+        const int step = static_cast<int>(w_pitch);
+        is_off1 = (min(r0 + g + 8, last) - min(r0 + g, last)) * step;
+        is_off2 = (min(r0 + g + 16, last) - min(r0 + g, last)) * step;
+        is_off3 = (min(r0 + g + 24, last) - min(r0 + g, last)) * step;
+        is_s = (b.w_row + min(r0 + g + 8 * t, last)) * groups;
+        is_wk = b.wk;
+        is_chunk = wk;
+        return;
       }
     };
-    auto issue_unit = [&]() {
-      // the scales queue moves up by one unit
-      q0 = q1;
-      q1 = q2;
-      q2 = q3;
-      r0 = r1;
-      r1 = r2;
-      r2 = r3;
-      if (is_step < steps) {
-        const int tile_row = (is_wn + is_tile * (kStreamWarps >> is_b.wk_log2)) << 4;
-        const int k0 = is_chunk << 7;
-        const uint32_t dst = ring + is_slot * kStreamUnitBytes;
+    const uint32_t ring = smem + warp * (kStreamRing * kStreamUnitBytes);
+    const uint32_t piece = (lane >> 2) * 64 + ((t ^ ((g >> 1) & 3)) << 4);  // 64-byte rows, 16-byte pieces swizzled by row / 2
+    // scales and zero points of the two units in flight (the first of them the next one in use): of row g + 8 t, one per
+    // scale block
+    uint32_t s0[kBlocks], s1[kBlocks], z0[kBlocks], z1[kBlocks];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int r = g + 8 * i, j = t;
-          // rows behind the CTA's part and K behind the end are left as they are: what they hold meets nothing that is kept
-          if (tile_row + r < is_b.nrows && k0 + 32 * j < p.K)
-            stream_copy_16(dst + r * 64 + ((j ^ ((r >> 1) & 3)) << 4),
-                        p.wq + (is_b.w_row + tile_row + r) * w_pitch + ((k0 + 32 * j) >> 1));
-        }
-        const int kk = min(k0 + 32 * t, p.K - 32);
-        const int64_t last = is_b.w_row + is_b.nrows - 1;
-        const int64_t at0 = min(is_b.w_row + tile_row + g, last) * groups + kk / p.group;
-        const int64_t at1 = min(is_b.w_row + tile_row + g + 8, last) * groups + kk / p.group;
-        q3 = __ldg(p.scales + at0);
-        r3 = __ldg(p.scales + at1);
-        if (p.zeros) {
-          q3 |= static_cast<uint32_t>(__ldg(p.zeros + at0)) << 16;
-          r3 |= static_cast<uint32_t>(__ldg(p.zeros + at1)) << 16;
+    for (int i = 0; i < kBlocks; ++i) s0[i] = s1[i] = z0[i] = z1[i] = 0;
+    auto issue_unit = [&]() {
+#pragma unroll
+      for (int i = 0; i < kBlocks; ++i) {
+        s0[i] = s1[i];
+        z0[i] = z1[i];
+      }
+      if (is_batch < count) {
+        // K behind the end: the last 32 again; those blocks are not used
+        const uint8_t* src = is_w + (min(is_chunk * 4 + t, last_block) << 4);
+        const uint32_t dst = ring + is_slot * kStreamUnitBytes + piece;
+        stream_copy_16(dst, src);
+        stream_copy_16(dst + 512, src + is_off1);
+        stream_copy_16(dst + 1024, src + is_off2);
+        stream_copy_16(dst + 1536, src + is_off3);
+#pragma unroll
+        for (int i = 0; i < kBlocks; ++i) {
+          const uint32_t block = min(is_chunk * 4 + i * GQ, last_block);
+          const int64_t at = is_s + (group_blocks > 1 ? __umulhi(block, magic) : block);
+          s1[i] = __ldg(p.scales + at);
+          if (p.zeros) z1[i] = __ldg(p.zeros + at);
         }
         if (++is_slot == kStreamRing) is_slot = 0;
-        if (++is_tile == is_tiles) {
-          is_tile = 0;
-          is_chunk += 1 << is_b.wk_log2;
-          if (is_chunk >= is_chunks) issue_step();
-        }
-      }
-      stream_commit();
-    };
-    auto stage_acts = [&](int step) {
-      const int b = step / slices, s = step - b * slices;
-      const int k0 = s * kSliceK, kn = min(kSliceK, p.K - k0);
-      const int a_row = batches[b].a_row, mrows = batches[b].mrows;
-      const uint32_t dst = smem + (step & 1) * kStreamActBytes;
-      uint8_t* dst_gen = smem_raw + (step & 1) * kStreamActBytes;
-      if (acts_aligned) {
-        const int pieces = kn >> 3;  // 16-byte pieces per row
-        for (int i = tid; i < mrows * pieces; i += kStreamThreads) {
-          const int m = i / pieces, c = i - m * pieces;
-          stream_copy_16(dst + m * kActPitch + c * 16, p.a + static_cast<int64_t>(a_row + m) * p.lda + k0 + c * 8);
-        }
-      } else {
-        for (int i = tid; i < mrows * kn; i += kStreamThreads) {
-          const int m = i / kn, c = i - m * kn;
-          *reinterpret_cast<uint16_t*>(dst_gen + m * kActPitch + c * 2) =
-              p.a[static_cast<int64_t>(a_row + m) * p.lda + k0 + c];
-        }
+        is_chunk += is_wk;
+        if (is_chunk >= chunks) issue_batch();
       }
       stream_commit();
     };
 
-    issue_step();
+    // ---- activations: copied as they are, then ordered and summed by the thread that copied them -------------------------
+    auto stage_acts = [&](int step) {
+      const int b = step / slices, s = step - b * slices;
+      const int k0 = s * slice_k, pieces = min(slice_k, p.K - k0) >> 3;  // 16-byte pieces per row
+      const int a_row = batches[b].a_row, mrows = batches[b].mrows;
+      const uint32_t dst = smem + kActOffset + (step & 1) * kStreamActBytes;
+      if (acts_aligned) {
+        for (int i = tid; i < mrows * pieces; i += kStreamThreads) {
+          const int m = i / pieces, c = i - m * pieces;
+          stream_copy_16(dst + m * act_pitch + c * 16, p.a + static_cast<int64_t>(a_row + m) * p.lda + k0 + c * 8);
+        }
+      }
+      stream_commit();
+    };
+    auto order_acts = [&](int step) {
+      const int b = step / slices, s = step - b * slices;
+      const int k0 = s * slice_k, pieces = min(slice_k, p.K - k0) >> 3;
+      const int a_row = batches[b].a_row, mrows = batches[b].mrows;
+      const uint32_t act = smem + kActOffset + (step & 1) * kStreamActBytes;
+      float* sums = reinterpret_cast<float*>(smem_raw + kSumOffset + (step & 1) * kStreamSumBytes);
+      const int n = mrows * pieces, turns = (n + kStreamThreads - 1) / kStreamThreads;
+      for (int turn = 0; turn < turns; ++turn) {
+        const int i = turn * kStreamThreads + tid;  // 4 GQ neighbours hold one scale block: pieces is a multiple of that
+        const bool live = i < n;
+        const int m = live ? i / pieces : 0, c = live ? i - m * pieces : 0;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (live) {
+          if (acts_aligned) {
+            v = lds128(act + m * act_pitch + c * 16);
+          } else {
+            const uint16_t* src = p.a + static_cast<int64_t>(a_row + m) * p.lda + k0 + c * 8;
+            v.x = src[0] | static_cast<uint32_t>(src[1]) << 16;
+            v.y = src[2] | static_cast<uint32_t>(src[3]) << 16;
+            v.z = src[4] | static_cast<uint32_t>(src[5]) << 16;
+            v.w = src[6] | static_cast<uint32_t>(src[7]) << 16;
+          }
+        }
+        const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          sum += half_bits_to_float<BF16>(words[j] & 0xffffu) + half_bits_to_float<BF16>(words[j] >> 16);
+#pragma unroll
+        for (int d = 1; d < 4 * GQ; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+        if (live) {
+          // (a0, a4), (a2, a6), (a1, a5), (a3, a7)
+          sts128(act + m * act_pitch + c * 16,
+                 make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.x, v.z, 0x7632),
+                            __byte_perm(v.y, v.w, 0x7632)));
+          if (c % (4 * GQ) == 0) {
+            sums[(c / (4 * GQ)) * kCols + m] = sum;
+            sums[kStreamSumBytes / 8 + (c / (4 * GQ)) * kCols + m] = -above * sum;
+          }
+        }
+      }
+    };
+
+    issue_batch();
 #pragma unroll
     for (int i = 0; i < kStreamRing - 1; ++i) issue_unit();
     if (!waited) {  // matrix-vector product: weights and scales may be fetched ahead, activations may not
@@ -321,81 +346,66 @@ __device__ void stream_body(const StreamArgs& p) {
     stage_acts(0);
     int since = 0;  // groups committed after the activations that the next step needs
     int slot = 0;
-    float total_acc[TM][NB * 4];
+    float total_acc[2][NB * 4];
 
     for (int step = 0; step < steps; ++step) {
       const int bi = step / slices, s = step - bi * slices;
-      // this thread's pieces of the step's activations have landed ...
+      // this thread's pieces of the step's activations have landed; the step before last is done with their sums
       if (since == 0) stream_wait<0>();
       else if (since == 1) stream_wait<1>();
-      else if (since == 2) stream_wait<2>();
-      else stream_wait<3>();
-      __syncthreads();  // ... and everybody's; the buffer of the step before is free
+      else stream_wait<2>();
+      order_acts(step);
+      __syncthreads();  // everybody's pieces are in order; the buffer of the step before is free
       since = 0;
       if (step + 1 < steps) stage_acts(step + 1);
       const StreamBatch b = batches[bi];
-      const int wk_n = 1 << b.wk_log2, wn_n = kStreamWarps >> b.wk_log2;
-      const int wk = warp & (wk_n - 1), wn = warp >> b.wk_log2;
-      const int tiles = (b.nrows + 15) >> 4, my_tiles = (tiles - wn + wn_n - 1) / wn_n;
+      const int wk = warp / b.wn, wn = warp - wk * b.wn;
       if (s == 0) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-          for (int j = 0; j < NB * 4; ++j) total_acc[i][j] = 0.f;
+        for (int j = 0; j < NB * 4; ++j) total_acc[0][j] = total_acc[1][j] = 0.f;
       }
-      const int first = s * (kSliceK / 128), last = min(chunks, first + kSliceK / 128);
-      const uint32_t act_base = smem + (step & 1) * kStreamActBytes + g * kActPitch + t * 16;
-      if (my_tiles > 0) {
-        for (int c = first + wk; c < last; c += wk_n) {
+      const int first = s * slice_chunks, last = min(chunks, first + slice_chunks);
+      const bool two = wn * 32 + 16 < b.nrows;
+      if (wk < b.wk) {
+        const uint32_t act_base = smem + kActOffset + (step & 1) * kStreamActBytes + g * act_pitch + t * 16;
+        const uint32_t sum_base = smem + kSumOffset + (step & 1) * kStreamSumBytes + t * 8;
+        const uint32_t w_lane = ring + g * 64 + t * 4;
+        const uint32_t sw = (g >> 1) & 3;
+        // this warp's chunks of the slice: wk, wk + WK, ... over all of K
+        for (int c = first + (wk + b.wk - first % b.wk) % b.wk; c < last; c += b.wk) {
           const int qn = min(4, (p.K - (c << 7)) >> 5);  // 32-wide blocks that the chunk holds
-          // activation fragments of the chunk: (a0, a4), (a2, a6), (a1, a5), (a3, a7) of each lane's eight values
-          uint32_t bf[NB][4][4];
-          float sum[NB][kBlocks][2];
+          stream_wait<kStreamRing - 2>();
+          __syncwarp();
+          const uint32_t w_base = w_lane + slot * kStreamUnitBytes;
+          const uint32_t act_c = act_base + ((c - first) << 8);
+          const uint32_t sum_c = sum_base + (c - first) * kBlocks * (kCols * 4);
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            const bool live = nb * 8 + g < b.mrows;
+          for (int blk = 0; blk < kBlocks; ++blk) {
+            if (blk * GQ < qn) {
+              float acc[2][NB][4];
 #pragma unroll
-            for (int q = 0; q < 4; ++q) {
-              uint4 v = make_uint4(0, 0, 0, 0);
-              if (live && q < qn) v = lds128(act_base + nb * 8 * kActPitch + ((c - first) << 8) + (q << 6));
-              bf[nb][q][0] = __byte_perm(v.x, v.z, 0x5410);
-              bf[nb][q][1] = __byte_perm(v.y, v.w, 0x5410);
-              bf[nb][q][2] = __byte_perm(v.x, v.z, 0x7632);
-              bf[nb][q][3] = __byte_perm(v.y, v.w, 0x7632);
-            }
+              for (int nb = 0; nb < NB; ++nb) {
+                const float2 init = lds64f(sum_c + kStreamSumBytes / 2 + blk * (kCols * 4) + nb * 32);
 #pragma unroll
-            for (int blk = 0; blk < kBlocks; ++blk) {
-              float d[4] = {0.f, 0.f, 0.f, 0.f};
+                for (int i = 0; i < 2; ++i) {
+                  acc[i][nb][0] = acc[i][nb][2] = init.x;
+                  acc[i][nb][1] = acc[i][nb][3] = init.y;
+                }
+              }
 #pragma unroll
               for (int h = 0; h < GQ; ++h) {
                 const int q = blk * GQ + h;
-                mma_16816<BF16>(d, ones, ones, ones, ones, bf[nb][q][0], bf[nb][q][1]);
-                mma_16816<BF16>(d, ones, ones, ones, ones, bf[nb][q][2], bf[nb][q][3]);
-              }
-              sum[nb][blk][0] = d[0];
-              sum[nb][blk][1] = d[1];
-            }
-          }
+                uint4 bf[NB];
 #pragma unroll
-          for (int i = 0; i < TM; ++i) {
-            if (i < my_tiles) {
-              stream_wait<kStreamRing - 2>();
-              __syncwarp();
-              const uint32_t w_base = ring + slot * kStreamUnitBytes + g * 64 + t * 4;
-              const int sw = (g >> 1) & 3;
-              const uint32_t sc0 = q0, sc1 = r0;
+                for (int nb = 0; nb < NB; ++nb) {
+                  bf[nb] = make_uint4(0, 0, 0, 0);
+                  if (nb * 8 + g < b.mrows) bf[nb] = lds128(act_c + nb * 8 * act_pitch + (q << 6));
+                }
 #pragma unroll
-              for (int blk = 0; blk < kBlocks; ++blk) {
-                if (blk * GQ < qn) {
-                  float acc[NB][4];
-#pragma unroll
-                  for (int nb = 0; nb < NB; ++nb)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) acc[nb][j] = 0.f;
-#pragma unroll
-                  for (int h = 0; h < GQ; ++h) {
-                    const int q = blk * GQ + h;
-                    const uint32_t w0 = lds32(w_base + ((q ^ sw) << 4)), w1 = lds32(w_base + ((q ^ sw) << 4) + 512);
+                for (int i = 0; i < 2; ++i) {
+                  if (i == 0 || two) {
+                    const uint32_t at = w_base + i * 1024 + ((q ^ sw) << 4);
+                    const uint32_t w0 = lds32(at), w1 = lds32(at + 512);
                     // nibbles (0, 4), (2, 6) and (1, 5), (3, 7) of either row
                     const uint32_t a0 = and_xor(BF16 ? w0 : w0 << 4, mask, under), a1 = and_xor(BF16 ? w1 : w1 << 4, mask, under);
                     const uint32_t a2 = and_xor(w0 >> (BF16 ? 8 : 4), mask, under), a3 = and_xor(w1 >> (BF16 ? 8 : 4), mask, under);
@@ -403,44 +413,56 @@ __device__ void stream_body(const StreamArgs& p) {
                     const uint32_t c2 = and_xor(w0 >> (BF16 ? 12 : 8), mask, under), c3 = and_xor(w1 >> (BF16 ? 12 : 8), mask, under);
 #pragma unroll
                     for (int nb = 0; nb < NB; ++nb) {
-                      mma_16816<BF16>(acc[nb], a0, a1, a2, a3, bf[nb][q][0], bf[nb][q][1]);
-                      mma_16816<BF16>(acc[nb], c0, c1, c2, c3, bf[nb][q][2], bf[nb][q][3]);
-                    }
-                  }
-                  // lane t of a quad loaded the scale of the chunk's 32-wide block t
-                  const uint32_t e0 = GQ == 4 ? sc0 : __shfl_sync(0xffffffffu, sc0, (lane & 28) | (blk * GQ));
-                  const uint32_t e1 = GQ == 4 ? sc1 : __shfl_sync(0xffffffffu, sc1, (lane & 28) | (blk * GQ));
-                  const float s0 = half_bits_to_float<BF16>(e0 & 0xffffu);
-                  const float s1 = half_bits_to_float<BF16>(e1 & 0xffffu);
-                  const float z0 = z_base + (p.zeros ? half_bits_to_float<BF16>(e0 >> 16) : 8.f);
-                  const float z1 = z_base + (p.zeros ? half_bits_to_float<BF16>(e1 >> 16) : 8.f);
-#pragma unroll
-                  for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                      const float v = fmaf(j < 2 ? -z0 : -z1, sum[nb][blk][j & 1], acc[nb][j]);
-                      total_acc[i][nb * 4 + j] = fmaf(j < 2 ? s0 : s1, v, total_acc[i][nb * 4 + j]);
+                      mma_16816<BF16>(acc[i][nb], a0, a1, a2, a3, bf[nb].x, bf[nb].y);
+                      mma_16816<BF16>(acc[i][nb], c0, c1, c2, c3, bf[nb].z, bf[nb].w);
                     }
                   }
                 }
               }
-              if (++slot == kStreamRing) slot = 0;
-              __syncwarp();  // every lane has read the unit: its slot may be filled again
-              issue_unit();
-              ++since;
+              float2 sum[NB];
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+                sum[nb] = p.zeros ? lds64f(sum_c + blk * (kCols * 4) + nb * 32) : make_float2(0.f, 0.f);
+#pragma unroll
+              for (int i = 0; i < 2; ++i) {
+                if (i == 0 || two) {
+                  // lane t of a quad holds row g + 8 t: this tile's two rows are those of lanes 2 i and 2 i + 1
+#pragma unroll
+                  for (int half = 0; half < 2; ++half) {
+                    const int from = (lane & 28) | (2 * i + half);
+                    const float sc = half_bits_to_float<BF16>(__shfl_sync(0xffffffffu, s0[blk], from));
+                    if (p.zeros) {
+                      const float z = -half_bits_to_float<BF16>(__shfl_sync(0xffffffffu, z0[blk], from));
+#pragma unroll
+                      for (int nb = 0; nb < NB; ++nb) {
+                        acc[i][nb][2 * half] = fmaf(z, sum[nb].x, acc[i][nb][2 * half]);
+                        acc[i][nb][2 * half + 1] = fmaf(z, sum[nb].y, acc[i][nb][2 * half + 1]);
+                      }
+                    }
+#pragma unroll
+                    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                      for (int j = 0; j < 2; ++j)
+                        total_acc[i][nb * 4 + 2 * half + j] =
+                            fmaf(sc, acc[i][nb][2 * half + j], total_acc[i][nb * 4 + 2 * half + j]);
+                  }
+                }
+              }
             }
           }
+          if (++slot == kStreamRing) slot = 0;
+          __syncwarp();  // every lane has read the unit: its slot may be filled again
+          issue_unit();
+          ++since;
         }
       }
       if (s == slices - 1) {
-        // the WK partial sums of each tile meet, in order of K, in the buffer of this step's activations
-        __syncthreads();
-        float* red = reinterpret_cast<float*>(smem_raw + (step & 1) * kStreamActBytes);
-        constexpr int kTile = 8 * NB * kRedPitch;
+        // the WK partial sums of each tile meet, in order of K
+        float* red = reinterpret_cast<float*>(smem_raw + kRedOffset);
+        if (wk < b.wk) {
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-          if (i < my_tiles) {
-            float* dst = red + (wk * tiles + wn + i * wn_n) * kTile;
+          for (int i = 0; i < 2; ++i) {
+            float* dst = red + (wk * b.wn + wn) * 2 * kTile + i * kTile;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
@@ -449,12 +471,13 @@ __device__ void stream_body(const StreamArgs& p) {
           }
         }
         __syncthreads();
-        for (int i = tid; i < b.mrows * (tiles << 4); i += kStreamThreads) {
-          const int m = i / (tiles << 4), n = i - m * (tiles << 4);
+        const int span = b.wn * 32;  // rows of the batch, padded to pairs
+        for (int i = tid; i < b.mrows * span; i += kStreamThreads) {
+          const int m = i / span, n = i - m * span;
           if (n < b.nrows) {
             const float* src = red + (n >> 4) * kTile + m * kRedPitch + (n & 15);
             float v = 0.f;
-            for (int w = 0; w < wk_n; ++w) v += src[w * tiles * kTile];
+            for (int w = 0; w < b.wk; ++w) v += src[w * b.wn * 2 * kTile];
             uint16_t bits;
             if (BF16) bits = __bfloat16_as_ushort(__float2bfloat16_rn(v));
             else bits = __half_as_ushort(__float2half_rn(v));
