@@ -1762,8 +1762,8 @@ constexpr int kWtMaxDestinations = 8;
 // staging region of the pack / unpack kernels: 64 rows of at most 512 bytes, 16 bytes of padding per row
 constexpr uint32_t kTilingStageBytes = 64 * (2 * 256 + 16);
 
-// b200_w4a16_stream_*: 16 warps x 3 units of 2 KiB, two activation slices with their sums, partial sums, tables
-constexpr uint32_t kStreamSmemBytes = 16 * 3 * 2048 + 2 * (33 * 1024 + 2 * 4096) + 16 * 2 * 16 * 20 * 4 + 32 * 32 + 1025 * 4 + 60;
+// b200_w4a16_stream_*: 16 warps x (3 units of 2 KiB, 2 KiB of scales), two activation slices with their sums, tables
+constexpr uint32_t kStreamSmemBytes = 16 * (3 * 2048 + 2 * 1024) + 2 * (40 * 1024 + 4096) + 32 * 32 + 1025 * 4 + 60;
 // b200_w4a16_experts_*: 4 activation stages of 32 KiB, 6 raw stages of 8 KiB, 2 staging tiles of 16 KiB, barriers, tables
 constexpr uint32_t kExpertsSmemBytes = 1024 + 4 * 32768 + 6 * 8192 + 2 * 16384 + 512 + 2 * 1025 * 4 + 56;
 // b200_expert_route: per expert a next row, an offset and 16 warps' counts, and the rows of 512 slots

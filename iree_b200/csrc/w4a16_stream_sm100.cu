@@ -34,14 +34,14 @@ constexpr int kStreamThreads = 512;
 constexpr int kStreamWarps = kStreamThreads / 32;
 constexpr int kStreamRing = 3;                        // units per warp: two in flight, 64 KiB per SM, and the one in use
 constexpr int kStreamUnitBytes = 2048;                // 32 weight rows x 128 K
-constexpr int kStreamActBytes = 33 * 1024;            // one activation slice
-constexpr int kStreamSumBytes = 2 * 4096;             // its sums, and the sums times the offset of the unpacked nibbles
-constexpr int kStreamRedBytes = kStreamWarps * 2 * 16 * 20 * 4;  // partial sums of 16 warps x 32 rows x 16 activation rows
+constexpr int kStreamActBytes = 40 * 1024;            // one activation slice; later the partial sums of 16 warps x 32 rows
+constexpr int kStreamSumBytes = 4096;                 // its sums
+constexpr int kStreamScaleBytes = 1024;               // scales and zero points of 32 rows x 8 scale blocks
 constexpr int kStreamBatchMax = 32;                   // batches described at a time
 constexpr int kStreamMaxExperts = 1024;
 constexpr int kStreamTableBytes = kStreamBatchMax * 32 + (kStreamMaxExperts + 1) * 4 + 60;
-constexpr int kStreamSmemBytes = kStreamWarps * kStreamRing * kStreamUnitBytes + 2 * (kStreamActBytes + kStreamSumBytes) +
-                                 kStreamRedBytes + kStreamTableBytes;
+constexpr int kStreamSmemBytes = kStreamWarps * (kStreamRing * kStreamUnitBytes + 2 * kStreamScaleBytes) +
+                                 2 * (kStreamActBytes + kStreamSumBytes) + kStreamTableBytes;
 static_assert(kStreamSmemBytes <= 232448, "per-CTA shared memory limit");
 
 struct StreamBatch {
@@ -62,6 +62,16 @@ __device__ __forceinline__ void stream_commit() { asm volatile("cp.async.commit_
 template <int N>
 __device__ __forceinline__ void stream_wait() {
   asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ uint2 stream_lds64(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr));
+  return v;
+}
+__device__ __forceinline__ uint32_t stream_lds16(uint32_t addr) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
+  return v;
 }
 __device__ __forceinline__ uint32_t and_xor(uint32_t a, uint32_t b, uint32_t c) {
   uint32_t r;
@@ -106,14 +116,14 @@ __device__ void stream_body(const StreamArgs& p) {
   constexpr int kTile = 8 * NB * kRedPitch;
   constexpr int kBlocks = 4 / GQ;                  // scale blocks per chunk of 128 K
   constexpr int kCols = 8 * NB;
-  static_assert(kStreamWarps * 2 * kTile * 4 <= kStreamRedBytes, "partial sums");
+  static_assert(kStreamWarps * 2 * kTile * 4 <= kStreamActBytes, "partial sums");
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t smem = smem_u32(smem_raw);
-  constexpr int kActOffset = kStreamWarps * kStreamRing * kStreamUnitBytes;
+  constexpr int kScaleOffset = kStreamWarps * kStreamRing * kStreamUnitBytes;
+  constexpr int kActOffset = kScaleOffset + kStreamWarps * 2 * kStreamScaleBytes;
   constexpr int kSumOffset = kActOffset + 2 * kStreamActBytes;
-  constexpr int kRedOffset = kSumOffset + 2 * kStreamSumBytes;
-  constexpr int kTableOffset = kRedOffset + kStreamRedBytes;
+  constexpr int kTableOffset = kSumOffset + 2 * kStreamSumBytes;
   StreamBatch* batches = reinterpret_cast<StreamBatch*>(smem_raw + kTableOffset);
   int* seg_first = reinterpret_cast<int*>(smem_raw + kTableOffset + kStreamBatchMax * 32);  // passes before each expert
   int* shared_words = seg_first + kStreamMaxExperts + 1;                                    // [0] batches in the table
@@ -122,13 +132,16 @@ __device__ void stream_body(const StreamArgs& p) {
   const int chunks = (p.K + 127) >> 7;
   // A slice holds the rows of one pass: as much of K as fits the buffers, in whole chunks.
   const int pass_rows = min(p.M, kCols);
-  const int most_k = min((kStreamActBytes / pass_rows - 64) >> 1, (kStreamSumBytes / 2) / (4 * kCols) * 32 * GQ);
+  const int most_k = min((kStreamActBytes / pass_rows - 64) >> 1, kStreamSumBytes / (4 * kCols) * 32 * GQ);
   const int fewest = (p.K + (most_k & ~127) - 1) / (most_k & ~127);
   const int slice_chunks = (chunks + fewest - 1) / fewest, slices = (chunks + slice_chunks - 1) / slice_chunks;
   const int slice_k = slice_chunks << 7;
   const int act_pitch = slice_k * 2 + 64;          // bytes; 64 mod 128: eight lanes of a 16-byte read hit all banks
   const bool acts_aligned = !((reinterpret_cast<uintptr_t>(p.a) | (static_cast<uintptr_t>(p.lda) * 2)) & 15);
   const int groups = p.K / p.group;
+  // Eight scale blocks of a row are 16 bytes to copy, or have to be picked one by one.
+  const bool scales_aligned = p.group == 32 * GQ && groups % 8 == 0 &&
+                              !((reinterpret_cast<uintptr_t>(p.scales) | reinterpret_cast<uintptr_t>(p.zeros)) & 15);
   // block of 32 K -> scale group without a division: exact for (K / 32) (group / 32) < 2^32
   const uint32_t group_blocks = static_cast<uint32_t>(p.group) >> 5;
   const uint32_t magic = group_blocks > 1 ? 0xffffffffu / group_blocks + 1u : 0u;
@@ -221,60 +234,74 @@ __device__ void stream_body(const StreamArgs& p) {
     for (int i = 0; i < count; ++i) row += batches[i].nrows;
     const int steps = count * slices;
 
-    // ---- unit sequence of this warp: (batch, chunk = wk, wk + WK, ...), ahead of its use ---------------------------------
-    int is_batch = -1, is_chunk = chunks, is_wk = 0, is_slot = 0;
-    const uint8_t* is_w = nullptr;       // this lane's 16 bytes of row g of the pair, K = 0
+    // ---- unit sequence of this warp: (batch, slice, its run of the slice's chunks), ahead of its use -----------------------
+    int is_batch = -1, is_slice = slices, is_chunk = 0, is_end = 0, is_super = -1;
+    uint32_t is_slot = 0, is_scales = 0;  // ring slot, and which of the two scale slots is filled next
+    int is_wk = 0, is_nwk = 1;
+    const uint8_t* is_w = nullptr;        // this lane's 16 bytes of row g of the pair, K = 0
     int32_t is_off1 = 0, is_off2 = 0, is_off3 = 0;  // bytes from there to rows g + 8, g + 16, g + 24 (the last row for rows behind it)
-    int64_t is_s = 0;                    // first scale of row g + 8 t
-    auto issue_batch = [&]() {  // the next batch in which this warp has a unit
-      while (++is_batch < count) {
-        const StreamBatch b = batches[is_batch];
-        const int wk = warp / b.wn, wn = warp - wk * b.wn;
-        if (wk >= b.wk || wk >= chunks) continue;
-        const int r0 = wn * 32, last = b.nrows - 1;
-        const int64_t first = b.w_row + min(r0 + g, last);
-        is_w = p.wq + first * w_pitch;
-        const int step = static_cast<int>(w_pitch);
-        is_off1 = (min(r0 + g + 8, last) - min(r0 + g, last)) * step;
-        is_off2 = (min(r0 + g + 16, last) - min(r0 + g, last)) * step;
-        is_off3 = (min(r0 + g + 24, last) - min(r0 + g, last)) * step;
-        is_s = (b.w_row + min(r0 + g + 8 * t, last)) * groups;
-        is_wk = b.wk;
-        is_chunk = wk;
-        return;
+    int64_t is_s = 0;                     // first scale of row `lane` of the pair
+    auto issue_run = [&]() {  // the next run of chunks that this warp has
+      while (is_batch < count) {
+        if (++is_slice >= slices) {
+          is_slice = 0;
+          if (++is_batch >= count) return;
+          const StreamBatch b = batches[is_batch];
+          const int wk = warp / b.wn, wn = warp - wk * b.wn;
+          const int r0 = wn * 32, last = b.nrows - 1, step = static_cast<int>(w_pitch);
+          is_w = p.wq + (b.w_row + min(r0 + g, last)) * w_pitch + t * 16;
+          is_off1 = (min(r0 + g + 8, last) - min(r0 + g, last)) * step;
+          is_off2 = (min(r0 + g + 16, last) - min(r0 + g, last)) * step;
+          is_off3 = (min(r0 + g + 24, last) - min(r0 + g, last)) * step;
+          is_s = (b.w_row + min(r0 + lane, last)) * groups;
+          is_wk = wk;
+          is_nwk = b.wk;
+        }
+        if (is_wk >= is_nwk) continue;
+        const int first = is_slice * slice_chunks, n = min(chunks - first, slice_chunks), per = (n + is_nwk - 1) / is_nwk;
+        is_chunk = first + is_wk * per;
+        is_end = min(is_chunk + per, first + n);
+        is_super = -1;
+        if (is_chunk < is_end) return;
       }
     };
     const uint32_t ring = smem + warp * (kStreamRing * kStreamUnitBytes);
-    const uint32_t piece = (lane >> 2) * 64 + ((t ^ ((g >> 1) & 3)) << 4);  // 64-byte rows, 16-byte pieces swizzled by row / 2
-    // scales and zero points of the two units in flight (the first of them the next one in use): of row g + 8 t, one per
-    // scale block
-    uint32_t s0[kBlocks], s1[kBlocks], z0[kBlocks], z1[kBlocks];
-#pragma unroll
-    for (int i = 0; i < kBlocks; ++i) s0[i] = s1[i] = z0[i] = z1[i] = 0;
+    const uint32_t scale_ring = smem + kScaleOffset + warp * (2 * kStreamScaleBytes);
+    const uint32_t ring_piece = ring + (lane >> 2) * 64 + ((t ^ ((g >> 1) & 3)) << 4);  // 64-byte rows, pieces swizzled by row / 2
     auto issue_unit = [&]() {
-#pragma unroll
-      for (int i = 0; i < kBlocks; ++i) {
-        s0[i] = s1[i];
-        z0[i] = z1[i];
-      }
       if (is_batch < count) {
-        // K behind the end: the last 32 again; those blocks are not used
-        const uint8_t* src = is_w + (min(is_chunk * 4 + t, last_block) << 4);
-        const uint32_t dst = ring + is_slot * kStreamUnitBytes + piece;
-        stream_copy_16(dst, src);
-        stream_copy_16(dst + 512, src + is_off1);
-        stream_copy_16(dst + 1024, src + is_off2);
-        stream_copy_16(dst + 1536, src + is_off3);
-#pragma unroll
-        for (int i = 0; i < kBlocks; ++i) {
-          const uint32_t block = min(is_chunk * 4 + i * GQ, last_block);
-          const int64_t at = is_s + (group_blocks > 1 ? __umulhi(block, magic) : block);
-          s1[i] = __ldg(p.scales + at);
-          if (p.zeros) z1[i] = __ldg(p.zeros + at);
+        if (is_chunk * 4 + t <= last_block) {  // K behind the end: what the slot holds meets zeros
+          const uint8_t* src = is_w + (static_cast<int64_t>(is_chunk) << 6);
+          const uint32_t dst = ring_piece + is_slot;
+          stream_copy_16(dst, src);
+          stream_copy_16(dst + 512, src + is_off1);
+          stream_copy_16(dst + 1024, src + is_off2);
+          stream_copy_16(dst + 1536, src + is_off3);
         }
-        if (++is_slot == kStreamRing) is_slot = 0;
-        is_chunk += is_wk;
-        if (is_chunk >= chunks) issue_batch();
+        is_slot = is_slot == (kStreamRing - 1) * kStreamUnitBytes ? 0 : is_slot + kStreamUnitBytes;
+        if (is_chunk / (2 * GQ) != is_super) {  // the next eight scale blocks of this lane's row
+          is_super = is_chunk / (2 * GQ);
+          const uint32_t dst = scale_ring + is_scales + lane * 16;
+          is_scales ^= kStreamScaleBytes;
+          if (scales_aligned) {
+            stream_copy_16(dst, p.scales + is_s + is_super * 8);
+            if (p.zeros) stream_copy_16(dst + 512, p.zeros + is_s + is_super * 8);
+          } else {
+            uint32_t sw[4] = {0, 0, 0, 0}, zw[4] = {0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              const uint32_t block = (is_super * 8 + i) * GQ;
+              if (block <= static_cast<uint32_t>(last_block)) {
+                const int64_t at = is_s + (group_blocks > 1 ? __umulhi(block, magic) : block);
+                sw[i >> 1] |= static_cast<uint32_t>(__ldg(p.scales + at)) << ((i & 1) * 16);
+                if (p.zeros) zw[i >> 1] |= static_cast<uint32_t>(__ldg(p.zeros + at)) << ((i & 1) * 16);
+              }
+            }
+            sts128(dst, make_uint4(sw[0], sw[1], sw[2], sw[3]));
+            if (p.zeros) sts128(dst + 512, make_uint4(zw[0], zw[1], zw[2], zw[3]));
+          }
+        }
+        if (++is_chunk >= is_end) issue_run();
       }
       stream_commit();
     };
@@ -283,12 +310,13 @@ __device__ void stream_body(const StreamArgs& p) {
     auto stage_acts = [&](int step) {
       const int b = step / slices, s = step - b * slices;
       const int k0 = s * slice_k, pieces = min(slice_k, p.K - k0) >> 3;  // 16-byte pieces per row
+      const int padded = (pieces + 15) & ~15;
       const int a_row = batches[b].a_row, mrows = batches[b].mrows;
       const uint32_t dst = smem + kActOffset + (step & 1) * kStreamActBytes;
       if (acts_aligned) {
-        for (int i = tid; i < mrows * pieces; i += kStreamThreads) {
-          const int m = i / pieces, c = i - m * pieces;
-          stream_copy_16(dst + m * act_pitch + c * 16, p.a + static_cast<int64_t>(a_row + m) * p.lda + k0 + c * 8);
+        for (int i = tid; i < mrows * padded; i += kStreamThreads) {
+          const int m = i / padded, c = i - m * padded;
+          if (c < pieces) stream_copy_16(dst + m * act_pitch + c * 16, p.a + static_cast<int64_t>(a_row + m) * p.lda + k0 + c * 8);
         }
       }
       stream_commit();
@@ -296,16 +324,17 @@ __device__ void stream_body(const StreamArgs& p) {
     auto order_acts = [&](int step) {
       const int b = step / slices, s = step - b * slices;
       const int k0 = s * slice_k, pieces = min(slice_k, p.K - k0) >> 3;
+      const int padded = (pieces + 15) & ~15;  // to whole chunks: zeros, which the last unit multiplies
       const int a_row = batches[b].a_row, mrows = batches[b].mrows;
       const uint32_t act = smem + kActOffset + (step & 1) * kStreamActBytes;
       float* sums = reinterpret_cast<float*>(smem_raw + kSumOffset + (step & 1) * kStreamSumBytes);
-      const int n = mrows * pieces, turns = (n + kStreamThreads - 1) / kStreamThreads;
+      const int n = mrows * padded, turns = (n + kStreamThreads - 1) / kStreamThreads;
       for (int turn = 0; turn < turns; ++turn) {
-        const int i = turn * kStreamThreads + tid;  // 4 GQ neighbours hold one scale block: pieces is a multiple of that
+        const int i = turn * kStreamThreads + tid;  // 4 GQ neighbours hold one scale block
         const bool live = i < n;
-        const int m = live ? i / pieces : 0, c = live ? i - m * pieces : 0;
+        const int m = live ? i / padded : 0, c = live ? i - m * padded : 0;
         uint4 v = make_uint4(0, 0, 0, 0);
-        if (live) {
+        if (live && c < pieces) {
           if (acts_aligned) {
             v = lds128(act + m * act_pitch + c * 16);
           } else {
@@ -328,15 +357,12 @@ __device__ void stream_body(const StreamArgs& p) {
           sts128(act + m * act_pitch + c * 16,
                  make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.x, v.z, 0x7632),
                             __byte_perm(v.y, v.w, 0x7632)));
-          if (c % (4 * GQ) == 0) {
-            sums[(c / (4 * GQ)) * kCols + m] = sum;
-            sums[kStreamSumBytes / 8 + (c / (4 * GQ)) * kCols + m] = -above * sum;
-          }
+          if (c % (4 * GQ) == 0) sums[(c / (4 * GQ)) * kCols + m] = sum;
         }
       }
     };
 
-    issue_batch();
+    issue_run();
 #pragma unroll
     for (int i = 0; i < kStreamRing - 1; ++i) issue_unit();
     if (!waited) {  // matrix-vector product: weights and scales may be fetched ahead, activations may not
@@ -345,12 +371,12 @@ __device__ void stream_body(const StreamArgs& p) {
     }
     stage_acts(0);
     int since = 0;  // groups committed after the activations that the next step needs
-    int slot = 0;
+    uint32_t slot = 0, scale_slot = kStreamScaleBytes;
     float total_acc[2][NB * 4];
 
     for (int step = 0; step < steps; ++step) {
       const int bi = step / slices, s = step - bi * slices;
-      // this thread's pieces of the step's activations have landed; the step before last is done with their sums
+      // this thread's pieces of the step's activations have landed
       if (since == 0) stream_wait<0>();
       else if (since == 1) stream_wait<1>();
       else stream_wait<2>();
@@ -364,101 +390,115 @@ __device__ void stream_body(const StreamArgs& p) {
 #pragma unroll
         for (int j = 0; j < NB * 4; ++j) total_acc[0][j] = total_acc[1][j] = 0.f;
       }
-      const int first = s * slice_chunks, last = min(chunks, first + slice_chunks);
-      const bool two = wn * 32 + 16 < b.nrows;
       if (wk < b.wk) {
-        const uint32_t act_base = smem + kActOffset + (step & 1) * kStreamActBytes + g * act_pitch + t * 16;
-        const uint32_t sum_base = smem + kSumOffset + (step & 1) * kStreamSumBytes + t * 8;
-        const uint32_t w_lane = ring + g * 64 + t * 4;
+        const int first = s * slice_chunks, n = min(chunks - first, slice_chunks), per = (n + b.wk - 1) / b.wk;
+        const int end = min(first + (wk + 1) * per, first + n);
+        // Columns behind the last activation row repeat rows that there are: what comes out of them is not stored.
+        uint32_t act_c[NB], sum_c = smem + kSumOffset + (step & 1) * kStreamSumBytes + t * 8 + wk * per * kBlocks * (kCols * 4);
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+          act_c[nb] = smem + kActOffset + (step & 1) * kStreamActBytes + min(nb * 8 + g, b.mrows - 1) * act_pitch + t * 16 +
+                      ((wk * per) << 8);
         const uint32_t sw = (g >> 1) & 3;
-        // this warp's chunks of the slice: wk, wk + WK, ... over all of K
-        for (int c = first + (wk + b.wk - first % b.wk) % b.wk; c < last; c += b.wk) {
-          const int qn = min(4, (p.K - (c << 7)) >> 5);  // 32-wide blocks that the chunk holds
+        const uint32_t w_lane = ring + g * 64 + t * 4;
+        const uint32_t w_at[4] = {w_lane + (sw << 4), w_lane + ((1 ^ sw) << 4), w_lane + ((2 ^ sw) << 4), w_lane + ((3 ^ sw) << 4)};
+        int super = -1;
+        for (int c = first + wk * per; c < end; ++c) {
           stream_wait<kStreamRing - 2>();
           __syncwarp();
-          const uint32_t w_base = w_lane + slot * kStreamUnitBytes;
-          const uint32_t act_c = act_base + ((c - first) << 8);
-          const uint32_t sum_c = sum_base + (c - first) * kBlocks * (kCols * 4);
+          if (c / (2 * GQ) != super) {
+            super = c / (2 * GQ);
+            scale_slot ^= kStreamScaleBytes;
+          }
+          // scales and zero points of rows g, g + 8, g + 16, g + 24: the chunk's blocks are 8 / GQ bytes of each row
+          const uint32_t sc_at = scale_ring + scale_slot + g * 16 + (c % (2 * GQ)) * (8 / GQ);
+          uint32_t sc[4][GQ == 1 ? 2 : 1], zp[4][GQ == 1 ? 2 : 1];
+#pragma unroll
+          for (int r = 0; r < 4; ++r) {
+            if constexpr (GQ == 1) {
+              const uint2 v = stream_lds64(sc_at + r * 128);
+              sc[r][0] = v.x;
+              sc[r][1] = v.y;
+              if (p.zeros) {
+                const uint2 z = stream_lds64(sc_at + r * 128 + 512);
+                zp[r][0] = z.x;
+                zp[r][1] = z.y;
+              }
+            } else if constexpr (GQ == 2) {
+              sc[r][0] = lds32(sc_at + r * 128);
+              if (p.zeros) zp[r][0] = lds32(sc_at + r * 128 + 512);
+            } else {
+              sc[r][0] = stream_lds16(sc_at + r * 128);
+              if (p.zeros) zp[r][0] = stream_lds16(sc_at + r * 128 + 512);
+            }
+          }
 #pragma unroll
           for (int blk = 0; blk < kBlocks; ++blk) {
-            if (blk * GQ < qn) {
-              float acc[2][NB][4];
+            float acc[2][NB][4];
+            float2 sum[NB];
 #pragma unroll
-              for (int nb = 0; nb < NB; ++nb) {
-                const float2 init = lds64f(sum_c + kStreamSumBytes / 2 + blk * (kCols * 4) + nb * 32);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                  acc[i][nb][0] = acc[i][nb][2] = init.x;
-                  acc[i][nb][1] = acc[i][nb][3] = init.y;
-                }
-              }
-#pragma unroll
-              for (int h = 0; h < GQ; ++h) {
-                const int q = blk * GQ + h;
-                uint4 bf[NB];
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-                  bf[nb] = make_uint4(0, 0, 0, 0);
-                  if (nb * 8 + g < b.mrows) bf[nb] = lds128(act_c + nb * 8 * act_pitch + (q << 6));
-                }
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                  if (i == 0 || two) {
-                    const uint32_t at = w_base + i * 1024 + ((q ^ sw) << 4);
-                    const uint32_t w0 = lds32(at), w1 = lds32(at + 512);
-                    // nibbles (0, 4), (2, 6) and (1, 5), (3, 7) of either row
-                    const uint32_t a0 = and_xor(BF16 ? w0 : w0 << 4, mask, under), a1 = and_xor(BF16 ? w1 : w1 << 4, mask, under);
-                    const uint32_t a2 = and_xor(w0 >> (BF16 ? 8 : 4), mask, under), a3 = and_xor(w1 >> (BF16 ? 8 : 4), mask, under);
-                    const uint32_t c0 = and_xor(BF16 ? w0 >> 4 : w0, mask, under), c1 = and_xor(BF16 ? w1 >> 4 : w1, mask, under);
-                    const uint32_t c2 = and_xor(w0 >> (BF16 ? 12 : 8), mask, under), c3 = and_xor(w1 >> (BF16 ? 12 : 8), mask, under);
-#pragma unroll
-                    for (int nb = 0; nb < NB; ++nb) {
-                      mma_16816<BF16>(acc[i][nb], a0, a1, a2, a3, bf[nb].x, bf[nb].y);
-                      mma_16816<BF16>(acc[i][nb], c0, c1, c2, c3, bf[nb].z, bf[nb].w);
-                    }
-                  }
-                }
-              }
-              float2 sum[NB];
-#pragma unroll
-              for (int nb = 0; nb < NB; ++nb)
-                sum[nb] = p.zeros ? lds64f(sum_c + blk * (kCols * 4) + nb * 32) : make_float2(0.f, 0.f);
+            for (int nb = 0; nb < NB; ++nb) {
+              sum[nb] = lds64f(sum_c + blk * (kCols * 4) + nb * 32);
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
-                if (i == 0 || two) {
-                  // lane t of a quad holds row g + 8 t: this tile's two rows are those of lanes 2 i and 2 i + 1
+                acc[i][nb][0] = acc[i][nb][2] = -above * sum[nb].x;
+                acc[i][nb][1] = acc[i][nb][3] = -above * sum[nb].y;
+              }
+            }
 #pragma unroll
-                  for (int half = 0; half < 2; ++half) {
-                    const int from = (lane & 28) | (2 * i + half);
-                    const float sc = half_bits_to_float<BF16>(__shfl_sync(0xffffffffu, s0[blk], from));
-                    if (p.zeros) {
-                      const float z = -half_bits_to_float<BF16>(__shfl_sync(0xffffffffu, z0[blk], from));
+            for (int h = 0; h < GQ; ++h) {
+              const int q = blk * GQ + h;
+              uint4 bf[NB];
 #pragma unroll
-                      for (int nb = 0; nb < NB; ++nb) {
-                        acc[i][nb][2 * half] = fmaf(z, sum[nb].x, acc[i][nb][2 * half]);
-                        acc[i][nb][2 * half + 1] = fmaf(z, sum[nb].y, acc[i][nb][2 * half + 1]);
-                      }
-                    }
+              for (int nb = 0; nb < NB; ++nb) bf[nb] = lds128(act_c[nb] + (q << 6));
 #pragma unroll
-                    for (int nb = 0; nb < NB; ++nb)
+              for (int i = 0; i < 2; ++i) {
+                const uint32_t at = w_at[q] + slot + i * 1024;
+                const uint32_t w0 = lds32(at), w1 = lds32(at + 512);
+                // nibbles (0, 4), (2, 6) and (1, 5), (3, 7) of either row
+                const uint32_t a0 = and_xor(BF16 ? w0 : w0 << 4, mask, under), a1 = and_xor(BF16 ? w1 : w1 << 4, mask, under);
+                const uint32_t a2 = and_xor(w0 >> (BF16 ? 8 : 4), mask, under), a3 = and_xor(w1 >> (BF16 ? 8 : 4), mask, under);
+                const uint32_t c0 = and_xor(BF16 ? w0 >> 4 : w0, mask, under), c1 = and_xor(BF16 ? w1 >> 4 : w1, mask, under);
+                const uint32_t c2 = and_xor(w0 >> (BF16 ? 12 : 8), mask, under), c3 = and_xor(w1 >> (BF16 ? 12 : 8), mask, under);
 #pragma unroll
-                      for (int j = 0; j < 2; ++j)
-                        total_acc[i][nb * 4 + 2 * half + j] =
-                            fmaf(sc, acc[i][nb][2 * half + j], total_acc[i][nb * 4 + 2 * half + j]);
-                  }
+                for (int nb = 0; nb < NB; ++nb) {
+                  mma_16816<BF16>(acc[i][nb], a0, a1, a2, a3, bf[nb].x, bf[nb].y);
+                  mma_16816<BF16>(acc[i][nb], c0, c1, c2, c3, bf[nb].z, bf[nb].w);
                 }
               }
             }
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {  // rows g + 8 r: half r & 1 of tile r >> 1
+              const float scale = half_bits_to_float<BF16>((sc[r][blk >> 1] >> ((blk & 1) * 16)) & 0xffffu);
+              if (p.zeros) {
+                const float z = half_bits_to_float<BF16>((zp[r][blk >> 1] >> ((blk & 1) * 16)) & 0xffffu);
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                  acc[r >> 1][nb][2 * (r & 1)] = fmaf(-z, sum[nb].x, acc[r >> 1][nb][2 * (r & 1)]);
+                  acc[r >> 1][nb][2 * (r & 1) + 1] = fmaf(-z, sum[nb].y, acc[r >> 1][nb][2 * (r & 1) + 1]);
+                }
+              }
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+                  total_acc[r >> 1][nb * 4 + 2 * (r & 1) + j] =
+                      fmaf(scale, acc[r >> 1][nb][2 * (r & 1) + j], total_acc[r >> 1][nb * 4 + 2 * (r & 1) + j]);
+            }
           }
-          if (++slot == kStreamRing) slot = 0;
+          slot = slot == (kStreamRing - 1) * kStreamUnitBytes ? 0 : slot + kStreamUnitBytes;
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) act_c[nb] += 256;
+          sum_c += kBlocks * (kCols * 4);
           __syncwarp();  // every lane has read the unit: its slot may be filled again
           issue_unit();
           ++since;
         }
       }
       if (s == slices - 1) {
-        // the WK partial sums of each tile meet, in order of K
-        float* red = reinterpret_cast<float*>(smem_raw + kRedOffset);
+        // the WK partial sums of each tile meet, in order of K, where this step's activations were
+        __syncthreads();
+        float* red = reinterpret_cast<float*>(smem_raw + kActOffset + (step & 1) * kStreamActBytes);
         if (wk < b.wk) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
