@@ -1762,8 +1762,8 @@ constexpr int kWtMaxDestinations = 8;
 // staging region of the pack / unpack kernels: 64 rows of at most 512 bytes, 16 bytes of padding per row
 constexpr uint32_t kTilingStageBytes = 64 * (2 * 256 + 16);
 
-// b200_w4a16_stream_*: 16 warps x (3 units of 2 KiB, 2 KiB of scales), two activation slices with their sums, tables
-constexpr uint32_t kStreamSmemBytes = 16 * (3 * 2048 + 2 * 1024) + 2 * (40 * 1024 + 4096) + 32 * 32 + 1025 * 4 + 60;
+// b200_w4a16_stream_*: 16 warps x (2 units of 2 KiB, 2 KiB of scales), two activation slices with their sums, tables
+constexpr uint32_t kStreamSmemBytes = 16 * (2 * 2048 + 2 * 1024) + 2 * (54 * 1024 + 4096) + 2 * 1025 * 4 + 16 * 304;
 // b200_w4a16_experts_*: 4 activation stages of 32 KiB, 6 raw stages of 8 KiB, 2 staging tiles of 16 KiB, barriers, tables
 constexpr uint32_t kExpertsSmemBytes = 1024 + 4 * 32768 + 6 * 8192 + 2 * 16384 + 512 + 2 * 1025 * 4 + 56;
 // b200_expert_route: per expert a next row, an offset and 16 warps' counts, and the rows of 512 slots
@@ -2470,7 +2470,7 @@ extern "C" {
 
 static bool misaligned(const void* p, uintptr_t bytes) { return (reinterpret_cast<uintptr_t>(p) % bytes) != 0; }
 
-// One dispatch of the export `name`, which orders itself on the device.
+// One dispatch of the export `name`, which orders itself on the device; launched early.
 static iree_b200_status_t dispatch_named(iree_b200_context_t* context, const char* name, int binding_count,
                                          const void* const* pointers, int constant_count, const int32_t* constants,
                                          uint32_t grid_x, uint32_t grid_y = 1) {
@@ -2481,7 +2481,14 @@ static iree_b200_status_t dispatch_named(iree_b200_context_t* context, const cha
   for (int i = 0; i < binding_count; ++i) bindings[i] = {static_cast<uint32_t>(i), const_cast<void*>(pointers[i])};
   B200_RETURN_IF_ERROR(iree_hal_b200_command_buffer_push_descriptor_set(cb, 0, binding_count, bindings));
   B200_RETURN_IF_ERROR(iree_hal_b200_command_buffer_push_constants(cb, 0, constants, constant_count * sizeof(int32_t)));
-  return dispatch_self_ordering(context, ord, binding_count, constant_count, grid_x, grid_y);
+  // These kernels wait on the device for everything ahead of them before they touch global memory (weights included, unless
+  // the caller turned dispatch overlap on), so launching them early is no promise of the caller's: it only hides their launch.
+  const bool saved_overlap = cb->overlap;
+  cb->overlap = g_cu.cuLaunchKernelEx && g_cu.cuGraphAddDependencies_v2;
+  const iree_b200_status_t st = iree_hal_b200_command_buffer_dispatch(cb, context->executable, ord, binding_count,
+                                                                      constant_count, grid_x, grid_y, 1);
+  cb->overlap = saved_overlap;
+  return st;
 }
 
 static iree_b200_status_t stream_validate(int32_t kind, int64_t M, int32_t N, int32_t K, int32_t group, int32_t lda,
@@ -2513,10 +2520,11 @@ static iree_b200_status_t stream_dispatch(iree_b200_context_t* context, int32_t 
   const char* name = kind == IREE_B200_KIND_F16 ? (wide ? "b200_w4a16_stream_f16_r16" : "b200_w4a16_stream_f16_r8")
                                                 : (wide ? "b200_w4a16_stream_bf16_r16" : "b200_w4a16_stream_bf16_r8");
   const void* pointers[6] = {a, wq, scales, zeros, offsets, out};
-  const int32_t constants[7] = {M, N, K, group, lda, ldo, experts};
+  const int32_t weights_ahead = context->dispatch_overlap || context->command_buffer->overlap;
+  const int32_t constants[8] = {M, N, K, group, lda, ldo, experts, weights_ahead};
   const int sms = usable_sms(context);
   const int64_t most = static_cast<int64_t>(M) * N;  // passes <= M
-  return dispatch_named(context, name, 6, pointers, 7, constants, static_cast<uint32_t>(most < sms ? most : sms));
+  return dispatch_named(context, name, 6, pointers, 8, constants, static_cast<uint32_t>(most < sms ? most : sms));
 }
 
 iree_b200_status_t iree_b200_w4a16_matvec(iree_b200_context_t* context, const iree_b200_w4a16_matvec_params_t* params,
@@ -2633,7 +2641,7 @@ iree_b200_status_t iree_b200_w4a16_experts_run(iree_b200_context_t* context, con
   if (!context) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "context is NULL");
   if (!p.rows || !p.N) return IREE_B200_STATUS_OK;
   if (!tensor)
-    return stream_dispatch(context, p.kind, p.rows > 4 * p.experts, a, wq, scales, zeros, offsets, out, p.rows, p.N, p.K,
+    return stream_dispatch(context, p.kind, p.rows > 8 * p.experts, a, wq, scales, zeros, offsets, out, p.rows, p.N, p.K,
                            p.group_size, p.lda, p.ldo, p.experts);
   // at most one part per 256 rows, and one more per expert
   const int64_t parts = (p.rows + 255) / 256 + (p.rows < p.experts ? p.rows : p.experts);

@@ -30,30 +30,94 @@
 
 namespace b200 {
 
-constexpr int kStreamThreads = 512;
-constexpr int kStreamWarps = kStreamThreads / 32;
-constexpr int kStreamRing = 3;                        // units per warp: two in flight, 64 KiB per SM, and the one in use
-constexpr int kStreamUnitBytes = 2048;                // 32 weight rows x 128 K
-constexpr int kStreamActBytes = 40 * 1024;            // one activation slice; later the partial sums of 16 warps x 32 rows
-constexpr int kStreamSumBytes = 4096;                 // its sums
-constexpr int kStreamScaleBytes = 1024;               // scales and zero points of 32 rows x 8 scale blocks
-constexpr int kStreamBatchMax = 32;                   // batches described at a time
+constexpr int kStreamWarps = 16;
+constexpr int kStreamThreads = kStreamWarps * 32;
+constexpr int kStreamRing = 2;                     // units in flight per warp: 64 KiB per SM
+constexpr int kStreamUnitBytes = 2048;             // 32 weight rows x 128 K
+constexpr int kStreamScaleBytes = 1024;            // scales and zero points of 32 rows x 8 scale blocks, two slots per warp
+constexpr int kStreamActBytes = 54 * 1024;         // one activation slice; later the warps' partial sums
+constexpr int kStreamSumBytes = 4096;              // the slice's sums
 constexpr int kStreamMaxExperts = 1024;
-constexpr int kStreamTableBytes = kStreamBatchMax * 32 + (kStreamMaxExperts + 1) * 4 + 60;
-constexpr int kStreamSmemBytes = kStreamWarps * (kStreamRing * kStreamUnitBytes + 2 * kStreamScaleBytes) +
-                                 2 * (kStreamActBytes + kStreamSumBytes) + kStreamTableBytes;
+constexpr int kStreamScaleOffset = kStreamWarps * kStreamRing * kStreamUnitBytes;
+constexpr int kStreamActOffset = kStreamScaleOffset + kStreamWarps * 2 * kStreamScaleBytes;
+constexpr int kStreamSumOffset = kStreamActOffset + 2 * kStreamActBytes;
+constexpr int kStreamTableOffset = kStreamSumOffset + 2 * kStreamSumBytes;
+constexpr int kStreamWalkOffset = kStreamTableOffset + 2 * (kStreamMaxExperts + 1) * 4;
+constexpr int kStreamWalkBytes = 304;              // per warp
+constexpr int kStreamSmemBytes = kStreamWalkOffset + kStreamWarps * kStreamWalkBytes;
 static_assert(kStreamSmemBytes <= 232448, "per-CTA shared memory limit");
 
 struct StreamBatch {
-  int64_t w_row;    // first weight row, over all experts
-  int32_t n0;       // the same within the expert = first result column
-  int32_t nrows;    // weight rows
-  int32_t a_row;    // first activation row
-  int32_t mrows;    // activation rows
-  int32_t wn;       // warp columns = pairs of tiles
-  int32_t wk;       // warps along K of each
+  int64_t w_row;  // first weight row, over all experts
+  int n0;         // the same within the expert = first result column
+  int nrows;      // weight rows
+  int a_row;      // first activation row
+  int mrows;      // activation rows
+  int wn;         // warp columns = pairs of tiles
+  int wk;         // warps along K of each
 };
-static_assert(sizeof(StreamBatch) == 32, "table size");
+
+// A CTA's part of the list of weight rows, batch by batch.
+struct StreamList {
+  const int* pass_first;  // passes before each expert (experts only)
+  const int* row_first;   // activation rows before each expert
+  int64_t row, row_end;   // in the list
+  int64_t pass;
+  int N, M, experts, cols, n0, e;
+
+  __device__ void begin(int64_t from, int64_t to) {
+    row = from;
+    row_end = to;
+    pass = row < N ? 0 : (row >> 32 ? row / N : static_cast<uint32_t>(row) / static_cast<uint32_t>(N));
+    n0 = static_cast<int>(row - pass * N);
+    e = 0;
+    if (pass_first) {
+      int hi = experts;  // last expert whose first pass is <= pass
+      while (hi - e > 1) {
+        const int mid = (e + hi) >> 1;
+        if (pass_first[mid] <= pass) e = mid;
+        else hi = mid;
+      }
+    }
+  }
+  __device__ bool next(StreamBatch& b) {
+    if (row >= row_end) return false;
+    const int64_t left = min(row_end - row, static_cast<int64_t>(N - n0));
+    int first = 0, have = M, nth = static_cast<int>(pass);
+    if (pass_first) {
+      while (pass_first[e + 1] <= pass) ++e;
+      first = row_first[e];
+      have = row_first[e + 1] - first;
+      nth = static_cast<int>(pass) - pass_first[e];
+    }
+    // Pairs of tiles for the 16 warps: 1-5, 7, 8 or 13-16; other counts would leave over a fifth of the warps idle.
+    constexpr uint32_t kPairs = 0x1e1beu;
+    const int most = static_cast<int>(min(left + 31, static_cast<int64_t>(kStreamWarps * 32)) >> 5);
+    const int pairs = 31 - __clz(kPairs & ((2u << most) - 1u));
+    b.w_row = static_cast<int64_t>(e) * N + n0;
+    b.n0 = n0;
+    b.nrows = static_cast<int>(min(left, static_cast<int64_t>(pairs * 32)));
+    b.a_row = first + nth * cols;
+    b.mrows = min(cols, have - nth * cols);
+    b.wn = pairs;
+    b.wk = kStreamWarps / pairs;
+    row += b.nrows;
+    n0 += b.nrows;
+    if (n0 == N) {
+      n0 = 0;
+      ++pass;
+    }
+    return true;
+  }
+};
+
+// Where a warp stands in the list: where it issues copies, and where it computes. Kept in shared memory (a step in every
+// few thousand cycles reads it), advanced by lane 0.
+struct StreamWalk {
+  StreamList issue, compute;
+  StreamBatch issue_batch, batch[2];  // batch: the one in use and the next
+};
+static_assert(sizeof(StreamWalk) <= kStreamWalkBytes, "walk");
 
 __device__ __forceinline__ void stream_copy_16(uint32_t dst, const void* src) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
@@ -77,6 +141,30 @@ __device__ __forceinline__ uint32_t and_xor(uint32_t a, uint32_t b, uint32_t c) 
   uint32_t r;
   asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(a), "r"(b), "r"(c));  // (a & b) ^ c
   return r;
+}
+// d = a b + c, c being (c0, c1) in both rows.
+template <bool BF16>
+__device__ __forceinline__ void mma_16816_first(float (&d)[4], float c0, float c1, uint32_t a0, uint32_t a1, uint32_t a2,
+                                                uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (BF16) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %10, %11};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+  } else {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %10, %11};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1));
+  }
+}
+// Four 8 x 16-byte matrices: lane l gives the address of row l & 7 of matrix l >> 3 and receives 4 bytes of row l >> 2 of each.
+__device__ __forceinline__ uint4 ldmatrix_x4(uint32_t addr) {
+  uint4 v;
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+               : "r"(addr));
+  return v;
 }
 template <bool BF16>
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -107,6 +195,7 @@ struct StreamArgs {
   const int32_t* offsets;    // NULL: one expert that owns all rows
   uint16_t* out;
   int M, N, K, group, lda, ldo, experts;
+  int weights_ahead;         // weights and scales may be read before the dispatch ahead is complete
 };
 
 // NB: blocks of 8 activation rows a pass covers; GQ: 32-wide K blocks per scale application (group % (32 GQ) == 0).
@@ -120,13 +209,8 @@ __device__ void stream_body(const StreamArgs& p) {
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t smem = smem_u32(smem_raw);
-  constexpr int kScaleOffset = kStreamWarps * kStreamRing * kStreamUnitBytes;
-  constexpr int kActOffset = kScaleOffset + kStreamWarps * 2 * kStreamScaleBytes;
-  constexpr int kSumOffset = kActOffset + 2 * kStreamActBytes;
-  constexpr int kTableOffset = kSumOffset + 2 * kStreamSumBytes;
-  StreamBatch* batches = reinterpret_cast<StreamBatch*>(smem_raw + kTableOffset);
-  int* seg_first = reinterpret_cast<int*>(smem_raw + kTableOffset + kStreamBatchMax * 32);  // passes before each expert
-  int* shared_words = seg_first + kStreamMaxExperts + 1;                                    // [0] batches in the table
+  int* pass_first = reinterpret_cast<int*>(smem_raw + kStreamTableOffset);  // passes before each expert
+  int* row_first = pass_first + kStreamMaxExperts + 1;                       // activation rows before each expert
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int chunks = (p.K + 127) >> 7;
@@ -149,18 +233,18 @@ __device__ void stream_body(const StreamArgs& p) {
   const int64_t w_pitch = p.K >> 1;
 
   grid_launch_dependents();
+  if (p.offsets || !p.weights_ahead) grid_dependency_wait();
   // Experts: how many passes (8 NB activation rows each) each one needs comes from the dispatch ahead.
-  int passes = (p.M + kCols - 1) / kCols;
+  int64_t passes = (p.M + kCols - 1) / kCols;
   if (p.offsets) {
-    grid_dependency_wait();
     if (warp == 0) {
       int sum = 0;
       for (int e0 = 0; e0 < p.experts; e0 += 32) {
         const int e = e0 + lane;
-        int need = 0;
+        int lo = 0, need = 0;
         if (e < p.experts) {
-          const int lo = min(max(p.offsets[e], 0), p.M), hi = min(max(p.offsets[e + 1], lo), p.M);
-          need = (hi - lo + kCols - 1) / kCols;
+          lo = min(max(p.offsets[e], 0), p.M);
+          need = (min(max(p.offsets[e + 1], lo), p.M) - lo + kCols - 1) / kCols;
         }
         int incl = need;
 #pragma unroll
@@ -168,85 +252,55 @@ __device__ void stream_body(const StreamArgs& p) {
           const int v = __shfl_up_sync(0xffffffffu, incl, d);
           if (lane >= d) incl += v;
         }
-        if (e < p.experts) seg_first[e] = sum + incl - need;
+        if (e < p.experts) {
+          pass_first[e] = sum + incl - need;
+          row_first[e] = lo;
+        }
         sum += __shfl_sync(0xffffffffu, incl, 31);
       }
-      if (lane == 0) seg_first[p.experts] = sum;
+      if (lane == 0) {
+        pass_first[p.experts] = sum;
+        row_first[p.experts] = min(max(p.offsets[p.experts], 0), p.M);
+      }
     }
     __syncthreads();
-    passes = seg_first[p.experts];
+    passes = pass_first[p.experts];
   }
-  const int64_t total = static_cast<int64_t>(passes) * p.N;  // weight rows to be read, over all passes
-  const int64_t share = (total + gridDim.x - 1) / gridDim.x;
-  int64_t row = share * blockIdx.x;
-  const int64_t row_end = min(row + share, total);
-  bool waited = p.offsets != nullptr;
+  const int64_t total = passes * p.N;  // weight rows to be read, over all passes
+  const int64_t share = total >> 32 ? (total + gridDim.x - 1) / gridDim.x
+                                    : (static_cast<uint32_t>(total) + gridDim.x - 1) / gridDim.x;
+  StreamWalk& walk = *reinterpret_cast<StreamWalk*>(smem_raw + kStreamWalkOffset + warp * kStreamWalkBytes);
+  if (lane == 0) {
+    StreamList list = {p.offsets ? pass_first : nullptr, row_first, 0, 0, 0, p.N, p.M, p.experts, kCols, 0, 0};
+    list.begin(min(share * blockIdx.x, total), min(share * (blockIdx.x + 1), total));
+    walk.issue = list;
+    walk.compute = list;
+  }
+  __syncwarp();
   const uint32_t mask = BF16 ? 0x000f000fu : 0x00f000f0u;
   const uint32_t under = BF16 ? (p.zeros ? 0x43004300u : 0x43084308u) : (p.zeros ? 0x54005400u : 0x54805480u);
   // what the unpacked nibbles stand above their values: of all of them, or without the zero points
   const float above = (BF16 ? 128.f : 64.f) + (p.zeros ? 0.f : 8.f);
 
-  while (row < row_end) {  // one turn for up to kStreamBatchMax batches: one, unless the operands are very uneven
-    __syncthreads();
-    if (tid == 0) {
-      int count = 0, e = 0;
-      int64_t pass = total == p.N ? 0 : row / p.N;
-      if (p.offsets) {
-        int lo = 0, hi = p.experts;  // last expert whose first pass is <= pass
-        while (hi - lo > 1) {
-          const int mid = (lo + hi) >> 1;
-          if (seg_first[mid] <= pass) lo = mid;
-          else hi = mid;
-        }
-        e = lo;
-      }
-      int64_t r = row;
-      while (r < row_end && count < kStreamBatchMax) {
-        const int n0 = static_cast<int>(r - pass * p.N);
-        const int64_t left = min(row_end - r, static_cast<int64_t>(p.N - n0));
-        int first = 0, have = p.M, nth = static_cast<int>(pass);
-        if (p.offsets) {
-          while (seg_first[e + 1] <= pass) ++e;
-          first = min(max(p.offsets[e], 0), p.M);
-          have = min(max(p.offsets[e + 1], first), p.M) - first;
-          nth = static_cast<int>(pass) - seg_first[e];
-        }
-        // Pairs of tiles that leave few of the 16 warps idle: 1-5, 7, 8, 13-16; others are cut at 4 or 8 pairs.
-        int pairs = static_cast<int>(min(left + 31, static_cast<int64_t>(512)) >> 5);
-        if (pairs == 6) pairs = 4;
-        else if (pairs > 8 && pairs < 13) pairs = 8;
-        StreamBatch b;
-        b.w_row = static_cast<int64_t>(e) * p.N + n0;
-        b.n0 = n0;
-        b.nrows = static_cast<int>(min(left, static_cast<int64_t>(pairs * 32)));
-        b.a_row = first + nth * kCols;
-        b.mrows = min(kCols, have - nth * kCols);
-        b.wn = pairs;
-        b.wk = kStreamWarps / pairs;
-        batches[count++] = b;
-        r += b.nrows;
-        if (n0 + b.nrows == p.N) ++pass;
-      }
-      shared_words[0] = count;
-    }
-    __syncthreads();
-    const int count = shared_words[0];
-    for (int i = 0; i < count; ++i) row += batches[i].nrows;
-    const int steps = count * slices;
-
     // ---- unit sequence of this warp: (batch, slice, its run of the slice's chunks), ahead of its use -----------------------
-    int is_batch = -1, is_slice = slices, is_chunk = 0, is_end = 0, is_super = -1;
+    bool is_more = true;
+    int is_slice = slices, is_chunk = 0, is_end = 0, is_super = -1;
     uint32_t is_slot = 0, is_scales = 0;  // ring slot, and which of the two scale slots is filled next
     int is_wk = 0, is_nwk = 1;
     const uint8_t* is_w = nullptr;        // this lane's 16 bytes of row g of the pair, K = 0
     int32_t is_off1 = 0, is_off2 = 0, is_off3 = 0;  // bytes from there to rows g + 8, g + 16, g + 24 (the last row for rows behind it)
     int64_t is_s = 0;                     // first scale of row `lane` of the pair
     auto issue_run = [&]() {  // the next run of chunks that this warp has
-      while (is_batch < count) {
+      while (is_more) {
         if (++is_slice >= slices) {
           is_slice = 0;
-          if (++is_batch >= count) return;
-          const StreamBatch b = batches[is_batch];
+          __syncwarp();  // every lane has read the batch before
+          bool one_more = false;
+          if (lane == 0) one_more = walk.issue.next(walk.issue_batch);
+          __syncwarp();
+          is_more = __any_sync(0xffffffffu, one_more);
+          if (!is_more) return;
+          const StreamBatch& b = walk.issue_batch;
           const int wk = warp / b.wn, wn = warp - wk * b.wn;
           const int r0 = wn * 32, last = b.nrows - 1, step = static_cast<int>(w_pitch);
           is_w = p.wq + (b.w_row + min(r0 + g, last)) * w_pitch + t * 16;
@@ -266,10 +320,10 @@ __device__ void stream_body(const StreamArgs& p) {
       }
     };
     const uint32_t ring = smem + warp * (kStreamRing * kStreamUnitBytes);
-    const uint32_t scale_ring = smem + kScaleOffset + warp * (2 * kStreamScaleBytes);
+    const uint32_t scale_ring = smem + kStreamScaleOffset + warp * (2 * kStreamScaleBytes);
     const uint32_t ring_piece = ring + (lane >> 2) * 64 + ((t ^ ((g >> 1) & 3)) << 4);  // 64-byte rows, pieces swizzled by row / 2
     auto issue_unit = [&]() {
-      if (is_batch < count) {
+      if (is_more) {
         if (is_chunk * 4 + t <= last_block) {  // K behind the end: what the slot holds meets zeros
           const uint8_t* src = is_w + (static_cast<int64_t>(is_chunk) << 6);
           const uint32_t dst = ring_piece + is_slot;
@@ -306,39 +360,34 @@ __device__ void stream_body(const StreamArgs& p) {
       stream_commit();
     };
 
-    // ---- activations: copied as they are, then ordered and summed by the thread that copied them -------------------------
-    auto stage_acts = [&](int step) {
-      const int b = step / slices, s = step - b * slices;
-      const int k0 = s * slice_k, pieces = min(slice_k, p.K - k0) >> 3;  // 16-byte pieces per row
-      const int padded = (pieces + 15) & ~15;
-      const int a_row = batches[b].a_row, mrows = batches[b].mrows;
-      const uint32_t dst = smem + kActOffset + (step & 1) * kStreamActBytes;
-      if (acts_aligned) {
-        for (int i = tid; i < mrows * padded; i += kStreamThreads) {
-          const int m = i / padded, c = i - m * padded;
-          if (c < pieces) stream_copy_16(dst + m * act_pitch + c * 16, p.a + static_cast<int64_t>(a_row + m) * p.lda + k0 + c * 8);
-        }
+    // ---- activations: copied as they are, then ordered and summed by the thread that copied them. Warps share out the rows,
+    // and each row's 16-byte pieces (the slice's K, up to whole chunks) go to the lanes of its warps in order.
+    auto stage_acts = [&](const StreamBatch& b, int s, int buffer) {
+      const int k0 = s * slice_k, pieces = min(slice_k, p.K - k0) >> 3;
+      const int parts = kStreamWarps / b.mrows, part = warp / b.mrows, m = warp - part * b.mrows;
+      if (acts_aligned && part < parts) {
+        const uint32_t dst = smem + kStreamActOffset + buffer * kStreamActBytes + m * act_pitch;
+        const uint16_t* src = p.a + static_cast<int64_t>(b.a_row + m) * p.lda + k0;
+        for (int c = part * 32 + lane; c < pieces; c += parts * 32) stream_copy_16(dst + c * 16, src + c * 8);
       }
       stream_commit();
     };
-    auto order_acts = [&](int step) {
-      const int b = step / slices, s = step - b * slices;
+    auto order_acts = [&](const StreamBatch& b, int s, int buffer) {
       const int k0 = s * slice_k, pieces = min(slice_k, p.K - k0) >> 3;
       const int padded = (pieces + 15) & ~15;  // to whole chunks: zeros, which the last unit multiplies
-      const int a_row = batches[b].a_row, mrows = batches[b].mrows;
-      const uint32_t act = smem + kActOffset + (step & 1) * kStreamActBytes;
-      float* sums = reinterpret_cast<float*>(smem_raw + kSumOffset + (step & 1) * kStreamSumBytes);
-      const int n = mrows * padded, turns = (n + kStreamThreads - 1) / kStreamThreads;
-      for (int turn = 0; turn < turns; ++turn) {
-        const int i = turn * kStreamThreads + tid;  // 4 GQ neighbours hold one scale block
-        const bool live = i < n;
-        const int m = live ? i / padded : 0, c = live ? i - m * padded : 0;
+      const int parts = kStreamWarps / b.mrows, part = warp / b.mrows, m = warp - part * b.mrows;
+      if (part >= parts) return;
+      const uint32_t act = smem + kStreamActOffset + buffer * kStreamActBytes + m * act_pitch;
+      float* sums = reinterpret_cast<float*>(smem_raw + kStreamSumOffset + buffer * kStreamSumBytes) + m;
+      const uint16_t* row = p.a + static_cast<int64_t>(b.a_row + m) * p.lda + k0;
+      for (int c0 = part * 32; c0 < padded; c0 += parts * 32) {
+        const int c = c0 + lane;  // 4 GQ neighbouring lanes hold one scale block
         uint4 v = make_uint4(0, 0, 0, 0);
-        if (live && c < pieces) {
+        if (c < pieces) {
           if (acts_aligned) {
-            v = lds128(act + m * act_pitch + c * 16);
+            v = lds128(act + c * 16);
           } else {
-            const uint16_t* src = p.a + static_cast<int64_t>(a_row + m) * p.lda + k0 + c * 8;
+            const uint16_t* src = row + c * 8;
             v.x = src[0] | static_cast<uint32_t>(src[1]) << 16;
             v.y = src[2] | static_cast<uint32_t>(src[3]) << 16;
             v.z = src[4] | static_cast<uint32_t>(src[5]) << 16;
@@ -352,39 +401,50 @@ __device__ void stream_body(const StreamArgs& p) {
           sum += half_bits_to_float<BF16>(words[j] & 0xffffu) + half_bits_to_float<BF16>(words[j] >> 16);
 #pragma unroll
         for (int d = 1; d < 4 * GQ; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-        if (live) {
+        if (c < padded) {
           // (a0, a4), (a2, a6), (a1, a5), (a3, a7)
-          sts128(act + m * act_pitch + c * 16,
-                 make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.x, v.z, 0x7632),
-                            __byte_perm(v.y, v.w, 0x7632)));
-          if (c % (4 * GQ) == 0) sums[(c / (4 * GQ)) * kCols + m] = sum;
+          sts128(act + c * 16, make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.y, v.w, 0x5410),
+                                          __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x7632)));
+          if ((lane & (4 * GQ - 1)) == 0) sums[c / (4 * GQ) * kCols] = sum;
         }
       }
     };
 
     issue_run();
 #pragma unroll
-    for (int i = 0; i < kStreamRing - 1; ++i) issue_unit();
-    if (!waited) {  // matrix-vector product: weights and scales may be fetched ahead, activations may not
-      grid_dependency_wait();
-      waited = true;
-    }
-    stage_acts(0);
+    for (int i = 0; i < kStreamRing; ++i) issue_unit();
+    if (!p.offsets && p.weights_ahead) grid_dependency_wait();  // weights and scales were fetched ahead, activations may not be
+    int turn = 0;  // which of the two batches is in use
+    auto next_batch = [&](int into) {
+      __syncwarp();  // every lane has read what was there
+      bool one_more = false;
+      if (lane == 0) one_more = walk.compute.next(walk.batch[into]);
+      __syncwarp();
+      return __any_sync(0xffffffffu, one_more) != 0;
+    };
+    bool more = next_batch(0);
+    if (more) stage_acts(walk.batch[0], 0, 0);
     int since = 0;  // groups committed after the activations that the next step needs
+    int buffer = 0, s = 0;
     uint32_t slot = 0, scale_slot = kStreamScaleBytes;
     float total_acc[2][NB * 4];
 
-    for (int step = 0; step < steps; ++step) {
-      const int bi = step / slices, s = step - bi * slices;
+    while (more) {  // one step: a slice of a batch
+      const bool ends = s == slices - 1;
+      const StreamBatch& b = walk.batch[turn];
       // this thread's pieces of the step's activations have landed
       if (since == 0) stream_wait<0>();
       else if (since == 1) stream_wait<1>();
       else stream_wait<2>();
-      order_acts(step);
+      order_acts(b, s, buffer);
       __syncthreads();  // everybody's pieces are in order; the buffer of the step before is free
       since = 0;
-      if (step + 1 < steps) stage_acts(step + 1);
-      const StreamBatch b = batches[bi];
+      if (!ends) {
+        stage_acts(b, s + 1, buffer ^ 1);
+      } else {
+        more = next_batch(turn ^ 1);
+        if (more) stage_acts(walk.batch[turn ^ 1], 0, buffer ^ 1);
+      }
       const int wk = warp / b.wn, wn = warp - wk * b.wn;
       if (s == 0) {
 #pragma unroll
@@ -394,17 +454,17 @@ __device__ void stream_body(const StreamArgs& p) {
         const int first = s * slice_chunks, n = min(chunks - first, slice_chunks), per = (n + b.wk - 1) / b.wk;
         const int end = min(first + (wk + 1) * per, first + n);
         // Columns behind the last activation row repeat rows that there are: what comes out of them is not stored.
-        uint32_t act_c[NB], sum_c = smem + kSumOffset + (step & 1) * kStreamSumBytes + t * 8 + wk * per * kBlocks * (kCols * 4);
+        uint32_t act_c[NB], sum_c = smem + kStreamSumOffset + buffer * kStreamSumBytes + t * 8 + wk * per * kBlocks * (kCols * 4);
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb)
-          act_c[nb] = smem + kActOffset + (step & 1) * kStreamActBytes + min(nb * 8 + g, b.mrows - 1) * act_pitch + t * 16 +
+          act_c[nb] = smem + kStreamActOffset + buffer * kStreamActBytes + min(nb * 8 + g, b.mrows - 1) * act_pitch + t * 16 +
                       ((wk * per) << 8);
-        const uint32_t sw = (g >> 1) & 3;
-        const uint32_t w_lane = ring + g * 64 + t * 4;
+        const uint32_t sw = (lane >> 1) & 3;
+        const uint32_t w_lane = ring + lane * 64;
         const uint32_t w_at[4] = {w_lane + (sw << 4), w_lane + ((1 ^ sw) << 4), w_lane + ((2 ^ sw) << 4), w_lane + ((3 ^ sw) << 4)};
         int super = -1;
         for (int c = first + wk * per; c < end; ++c) {
-          stream_wait<kStreamRing - 2>();
+          stream_wait<kStreamRing - 1>();
           __syncwarp();
           if (c / (2 * GQ) != super) {
             super = c / (2 * GQ);
@@ -437,24 +497,17 @@ __device__ void stream_body(const StreamArgs& p) {
             float acc[2][NB][4];
             float2 sum[NB];
 #pragma unroll
-            for (int nb = 0; nb < NB; ++nb) {
-              sum[nb] = lds64f(sum_c + blk * (kCols * 4) + nb * 32);
-#pragma unroll
-              for (int i = 0; i < 2; ++i) {
-                acc[i][nb][0] = acc[i][nb][2] = -above * sum[nb].x;
-                acc[i][nb][1] = acc[i][nb][3] = -above * sum[nb].y;
-              }
-            }
+            for (int nb = 0; nb < NB; ++nb) sum[nb] = lds64f(sum_c + blk * (kCols * 4) + nb * 32);
 #pragma unroll
             for (int h = 0; h < GQ; ++h) {
               const int q = blk * GQ + h;
               uint4 bf[NB];
 #pragma unroll
               for (int nb = 0; nb < NB; ++nb) bf[nb] = lds128(act_c[nb] + (q << 6));
+              const uint4 w = ldmatrix_x4(w_at[q] + slot);  // rows g, g + 8, g + 16, g + 24
 #pragma unroll
               for (int i = 0; i < 2; ++i) {
-                const uint32_t at = w_at[q] + slot + i * 1024;
-                const uint32_t w0 = lds32(at), w1 = lds32(at + 512);
+                const uint32_t w0 = i ? w.z : w.x, w1 = i ? w.w : w.y;
                 // nibbles (0, 4), (2, 6) and (1, 5), (3, 7) of either row
                 const uint32_t a0 = and_xor(BF16 ? w0 : w0 << 4, mask, under), a1 = and_xor(BF16 ? w1 : w1 << 4, mask, under);
                 const uint32_t a2 = and_xor(w0 >> (BF16 ? 8 : 4), mask, under), a3 = and_xor(w1 >> (BF16 ? 8 : 4), mask, under);
@@ -462,7 +515,10 @@ __device__ void stream_body(const StreamArgs& p) {
                 const uint32_t c2 = and_xor(w0 >> (BF16 ? 12 : 8), mask, under), c3 = and_xor(w1 >> (BF16 ? 12 : 8), mask, under);
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
-                  mma_16816<BF16>(acc[i][nb], a0, a1, a2, a3, bf[nb].x, bf[nb].y);
+                  if (h == 0)
+                    mma_16816_first<BF16>(acc[i][nb], -above * sum[nb].x, -above * sum[nb].y, a0, a1, a2, a3, bf[nb].x, bf[nb].y);
+                  else
+                    mma_16816<BF16>(acc[i][nb], a0, a1, a2, a3, bf[nb].x, bf[nb].y);
                   mma_16816<BF16>(acc[i][nb], c0, c1, c2, c3, bf[nb].z, bf[nb].w);
                 }
               }
@@ -495,10 +551,10 @@ __device__ void stream_body(const StreamArgs& p) {
           ++since;
         }
       }
-      if (s == slices - 1) {
+      if (ends) {
         // the WK partial sums of each tile meet, in order of K, where this step's activations were
         __syncthreads();
-        float* red = reinterpret_cast<float*>(smem_raw + kActOffset + (step & 1) * kStreamActBytes);
+        float* red = reinterpret_cast<float*>(smem_raw + kStreamActOffset + buffer * kStreamActBytes);
         if (wk < b.wk) {
 #pragma unroll
           for (int i = 0; i < 2; ++i) {
@@ -524,11 +580,14 @@ __device__ void stream_body(const StreamArgs& p) {
             p.out[static_cast<int64_t>(b.a_row + m) * p.ldo + b.n0 + n] = bits;
           }
         }
+        turn ^= 1;
+        s = 0;
+      } else {
+        ++s;
       }
+      buffer ^= 1;
     }
     stream_wait<0>();
-  }
-  if (!waited) grid_dependency_wait();
 }
 
 template <bool BF16, int NB>
@@ -545,8 +604,8 @@ __device__ __forceinline__ void stream_by_group(const StreamArgs& p) {
 #define B200_W4A16_STREAM(NAME, BF16, NB)                                                                                 \
   extern "C" __global__ void __launch_bounds__(b200::kStreamThreads, 1)                                                   \
       NAME(const uint16_t* a, const uint8_t* wq, const uint16_t* scales, const uint16_t* zeros, const int32_t* offsets,   \
-           uint16_t* out, int M, int N, int K, int group, int lda, int ldo, int experts) {                                \
-    b200::StreamArgs p = {a, wq, scales, zeros, offsets, out, M, N, K, group, lda, ldo, experts};                         \
+           uint16_t* out, int M, int N, int K, int group, int lda, int ldo, int experts, int weights_ahead) {             \
+    b200::StreamArgs p = {a, wq, scales, zeros, offsets, out, M, N, K, group, lda, ldo, experts, weights_ahead};          \
     b200::stream_by_group<BF16, NB>(p);                                                                                   \
   }
 B200_W4A16_STREAM(b200_w4a16_stream_f16_r8, false, 1)
