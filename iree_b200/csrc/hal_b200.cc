@@ -1763,6 +1763,7 @@ constexpr int kWtMaxDestinations = 8;
 constexpr uint32_t kTilingStageBytes = 64 * (2 * 256 + 16);
 
 // b200_w4a16_stream_*: 16 warps x (2 units of 2 KiB, 2 KiB of scales), two activation slices with their sums, tables
+constexpr int kStreamActBytes = 54 * 1024, kStreamSumBytes = 4096;
 constexpr uint32_t kStreamSmemBytes = 16 * (2 * 2048 + 2 * 1024) + 2 * (54 * 1024 + 4096) + 2 * 1025 * 4 + 16 * 304;
 // b200_w4a16_experts_*: 4 activation stages of 32 KiB, 6 raw stages of 8 KiB, 2 staging tiles of 16 KiB, barriers, tables
 constexpr uint32_t kExpertsSmemBytes = 1024 + 4 * 32768 + 6 * 8192 + 2 * 16384 + 512 + 2 * 1025 * 4 + 56;
@@ -2520,11 +2521,20 @@ static iree_b200_status_t stream_dispatch(iree_b200_context_t* context, int32_t 
   const char* name = kind == IREE_B200_KIND_F16 ? (wide ? "b200_w4a16_stream_f16_r16" : "b200_w4a16_stream_f16_r8")
                                                 : (wide ? "b200_w4a16_stream_bf16_r16" : "b200_w4a16_stream_bf16_r8");
   const void* pointers[6] = {a, wq, scales, zeros, offsets, out};
+  // Activation slices: whole chunks of 128 K that the kernel's buffers hold for the rows of one pass, in equal parts.
+  const int cols = wide ? 16 : 8, rows = M < cols ? M : cols, chunks = (K + 127) / 128;
+  const int blocks = group % 128 == 0 ? 4 : group % 64 == 0 ? 2 : 1;  // 32-wide K blocks per sum
+  int most = (kStreamActBytes / rows - 64) / 2;
+  const int most_sums = kStreamSumBytes / (4 * cols) * 32 * blocks;
+  if (most > most_sums) most = most_sums;
+  most /= 128;
+  const int fewest = (chunks + most - 1) / most;
+  const int slice_chunks = (chunks + fewest - 1) / fewest, slices = (chunks + slice_chunks - 1) / slice_chunks;
   const int32_t weights_ahead = context->dispatch_overlap || context->command_buffer->overlap;
-  const int32_t constants[8] = {M, N, K, group, lda, ldo, experts, weights_ahead};
+  const int32_t constants[11] = {M, N, K, group, lda, ldo, experts, slice_chunks, slices, K / group, weights_ahead};
   const int sms = usable_sms(context);
-  const int64_t most = static_cast<int64_t>(M) * N;  // passes <= M
-  return dispatch_named(context, name, 6, pointers, 8, constants, static_cast<uint32_t>(most < sms ? most : sms));
+  const int64_t list = static_cast<int64_t>(M) * N;  // weight rows over all passes, at most
+  return dispatch_named(context, name, 6, pointers, 11, constants, static_cast<uint32_t>(list < sms ? list : sms));
 }
 
 iree_b200_status_t iree_b200_w4a16_matvec(iree_b200_context_t* context, const iree_b200_w4a16_matvec_params_t* params,

@@ -47,6 +47,11 @@ constexpr int kStreamWalkBytes = 304;              // per warp
 constexpr int kStreamSmemBytes = kStreamWalkOffset + kStreamWarps * kStreamWalkBytes;
 static_assert(kStreamSmemBytes <= 232448, "per-CTA shared memory limit");
 
+// a / b for 0 <= a < 2^16, 0 < b <= 2^10: (a + 1/2) / b is at least 1 / 2b from a whole number, far more than the error.
+__device__ __forceinline__ int small_div(int a, int b) {
+  return __float2int_rd((static_cast<float>(a) + 0.5f) * __frcp_rn(static_cast<float>(b)));
+}
+
 struct StreamBatch {
   int64_t w_row;  // first weight row, over all experts
   int n0;         // the same within the expert = first result column
@@ -100,7 +105,7 @@ struct StreamList {
     b.a_row = first + nth * cols;
     b.mrows = min(cols, have - nth * cols);
     b.wn = pairs;
-    b.wk = kStreamWarps / pairs;
+    b.wk = small_div(kStreamWarps, pairs);
     row += b.nrows;
     n0 += b.nrows;
     if (n0 == N) {
@@ -195,6 +200,8 @@ struct StreamArgs {
   const int32_t* offsets;    // NULL: one expert that owns all rows
   uint16_t* out;
   int M, N, K, group, lda, ldo, experts;
+  int slice_chunks, slices;  // chunks of 128 K per activation slice, and slices
+  int groups;                // K / group
   int weights_ahead;         // weights and scales may be read before the dispatch ahead is complete
 };
 
@@ -214,15 +221,12 @@ __device__ void stream_body(const StreamArgs& p) {
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
   const int chunks = (p.K + 127) >> 7;
-  // A slice holds the rows of one pass: as much of K as fits the buffers, in whole chunks.
-  const int pass_rows = min(p.M, kCols);
-  const int most_k = min((kStreamActBytes / pass_rows - 64) >> 1, kStreamSumBytes / (4 * kCols) * 32 * GQ);
-  const int fewest = (p.K + (most_k & ~127) - 1) / (most_k & ~127);
-  const int slice_chunks = (chunks + fewest - 1) / fewest, slices = (chunks + slice_chunks - 1) / slice_chunks;
+  // A slice holds the rows of one pass: as much of K as fits the buffers, in whole chunks (stream_slice of the host).
+  const int slice_chunks = p.slice_chunks, slices = p.slices;
   const int slice_k = slice_chunks << 7;
   const int act_pitch = slice_k * 2 + 64;          // bytes; 64 mod 128: eight lanes of a 16-byte read hit all banks
   const bool acts_aligned = !((reinterpret_cast<uintptr_t>(p.a) | (static_cast<uintptr_t>(p.lda) * 2)) & 15);
-  const int groups = p.K / p.group;
+  const int groups = p.groups;
   // Eight scale blocks of a row are 16 bytes to copy, or have to be picked one by one.
   const bool scales_aligned = p.group == 32 * GQ && groups % 8 == 0 &&
                               !((reinterpret_cast<uintptr_t>(p.scales) | reinterpret_cast<uintptr_t>(p.zeros)) & 15);
@@ -301,7 +305,7 @@ __device__ void stream_body(const StreamArgs& p) {
           is_more = __any_sync(0xffffffffu, one_more);
           if (!is_more) return;
           const StreamBatch& b = walk.issue_batch;
-          const int wk = warp / b.wn, wn = warp - wk * b.wn;
+          const int wk = small_div(warp, b.wn), wn = warp - wk * b.wn;
           const int r0 = wn * 32, last = b.nrows - 1, step = static_cast<int>(w_pitch);
           is_w = p.wq + (b.w_row + min(r0 + g, last)) * w_pitch + t * 16;
           is_off1 = (min(r0 + g + 8, last) - min(r0 + g, last)) * step;
@@ -312,7 +316,7 @@ __device__ void stream_body(const StreamArgs& p) {
           is_nwk = b.wk;
         }
         if (is_wk >= is_nwk) continue;
-        const int first = is_slice * slice_chunks, n = min(chunks - first, slice_chunks), per = (n + is_nwk - 1) / is_nwk;
+        const int first = is_slice * slice_chunks, n = min(chunks - first, slice_chunks), per = small_div(n + is_nwk - 1, is_nwk);
         is_chunk = first + is_wk * per;
         is_end = min(is_chunk + per, first + n);
         is_super = -1;
@@ -364,7 +368,7 @@ __device__ void stream_body(const StreamArgs& p) {
     // and each row's 16-byte pieces (the slice's K, up to whole chunks) go to the lanes of its warps in order.
     auto stage_acts = [&](const StreamBatch& b, int s, int buffer) {
       const int k0 = s * slice_k, pieces = min(slice_k, p.K - k0) >> 3;
-      const int parts = kStreamWarps / b.mrows, part = warp / b.mrows, m = warp - part * b.mrows;
+      const int parts = small_div(kStreamWarps, b.mrows), part = small_div(warp, b.mrows), m = warp - part * b.mrows;
       if (acts_aligned && part < parts) {
         const uint32_t dst = smem + kStreamActOffset + buffer * kStreamActBytes + m * act_pitch;
         const uint16_t* src = p.a + static_cast<int64_t>(b.a_row + m) * p.lda + k0;
@@ -375,7 +379,7 @@ __device__ void stream_body(const StreamArgs& p) {
     auto order_acts = [&](const StreamBatch& b, int s, int buffer) {
       const int k0 = s * slice_k, pieces = min(slice_k, p.K - k0) >> 3;
       const int padded = (pieces + 15) & ~15;  // to whole chunks: zeros, which the last unit multiplies
-      const int parts = kStreamWarps / b.mrows, part = warp / b.mrows, m = warp - part * b.mrows;
+      const int parts = small_div(kStreamWarps, b.mrows), part = small_div(warp, b.mrows), m = warp - part * b.mrows;
       if (part >= parts) return;
       const uint32_t act = smem + kStreamActOffset + buffer * kStreamActBytes + m * act_pitch;
       float* sums = reinterpret_cast<float*>(smem_raw + kStreamSumOffset + buffer * kStreamSumBytes) + m;
@@ -445,13 +449,13 @@ __device__ void stream_body(const StreamArgs& p) {
         more = next_batch(turn ^ 1);
         if (more) stage_acts(walk.batch[turn ^ 1], 0, buffer ^ 1);
       }
-      const int wk = warp / b.wn, wn = warp - wk * b.wn;
+      const int wk = small_div(warp, b.wn), wn = warp - wk * b.wn;
       if (s == 0) {
 #pragma unroll
         for (int j = 0; j < NB * 4; ++j) total_acc[0][j] = total_acc[1][j] = 0.f;
       }
       if (wk < b.wk) {
-        const int first = s * slice_chunks, n = min(chunks - first, slice_chunks), per = (n + b.wk - 1) / b.wk;
+        const int first = s * slice_chunks, n = min(chunks - first, slice_chunks), per = small_div(n + b.wk - 1, b.wk);
         const int end = min(first + (wk + 1) * per, first + n);
         // Columns behind the last activation row repeat rows that there are: what comes out of them is not stored.
         uint32_t act_c[NB], sum_c = smem + kStreamSumOffset + buffer * kStreamSumBytes + t * 8 + wk * per * kBlocks * (kCols * 4);
@@ -567,9 +571,9 @@ __device__ void stream_body(const StreamArgs& p) {
           }
         }
         __syncthreads();
-        const int span = b.wn * 32;  // rows of the batch, padded to pairs
-        for (int i = tid; i < b.mrows * span; i += kStreamThreads) {
-          const int m = i / span, n = i - m * span;
+        // a warp takes 32 columns of one activation row at a time
+        for (int i = warp; i < b.mrows * b.wn; i += kStreamWarps) {
+          const int m = small_div(i, b.wn), n = (i - m * b.wn) * 32 + lane;
           if (n < b.nrows) {
             const float* src = red + (n >> 4) * kTile + m * kRedPitch + (n & 15);
             float v = 0.f;
@@ -604,8 +608,10 @@ __device__ __forceinline__ void stream_by_group(const StreamArgs& p) {
 #define B200_W4A16_STREAM(NAME, BF16, NB)                                                                                 \
   extern "C" __global__ void __launch_bounds__(b200::kStreamThreads, 1)                                                   \
       NAME(const uint16_t* a, const uint8_t* wq, const uint16_t* scales, const uint16_t* zeros, const int32_t* offsets,   \
-           uint16_t* out, int M, int N, int K, int group, int lda, int ldo, int experts, int weights_ahead) {             \
-    b200::StreamArgs p = {a, wq, scales, zeros, offsets, out, M, N, K, group, lda, ldo, experts, weights_ahead};          \
+           uint16_t* out, int M, int N, int K, int group, int lda, int ldo, int experts, int slice_chunks, int slices,  \
+           int groups, int weights_ahead) {                                                                                \
+    b200::StreamArgs p = {a, wq, scales, zeros, offsets, out, M, N, K, group, lda, ldo, experts,                  \
+                          slice_chunks, slices, groups, weights_ahead};                                                    \
     b200::stream_by_group<BF16, NB>(p);                                                                                   \
   }
 B200_W4A16_STREAM(b200_w4a16_stream_f16_r8, false, 1)
