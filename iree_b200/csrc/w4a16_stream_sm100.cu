@@ -192,6 +192,14 @@ __device__ __forceinline__ float half_bits_to_float(uint32_t bits) {
   return __half2float(__ushort_as_half(static_cast<unsigned short>(bits)));
 }
 
+// An array's start, 256 bytes at most, on its way to L2, in whole 16-byte pieces inside the array.
+__device__ __forceinline__ void prefetch_l2(const void* base, int64_t bytes) {
+  const uintptr_t begin = (reinterpret_cast<uintptr_t>(base) + 15) & ~static_cast<uintptr_t>(15);
+  const uintptr_t end = (reinterpret_cast<uintptr_t>(base) + min(bytes, static_cast<int64_t>(256))) & ~static_cast<uintptr_t>(15);
+  if (begin < end)
+    asm volatile("cp.async.bulk.prefetch.L2.global [%0], %1;" ::"l"(begin), "r"(static_cast<uint32_t>(end - begin)) : "memory");
+}
+
 struct StreamArgs {
   const uint16_t* a;
   const uint8_t* wq;
@@ -237,7 +245,7 @@ __device__ void stream_body(const StreamArgs& p) {
   const int64_t w_pitch = p.K >> 1;
 
   grid_launch_dependents();
-  if (p.offsets || !p.weights_ahead) grid_dependency_wait();
+  if (p.offsets) grid_dependency_wait();
   // Experts: how many passes (8 NB activation rows each) each one needs comes from the dispatch ahead.
   int64_t passes = (p.M + kCols - 1) / kCols;
   if (p.offsets) {
@@ -281,6 +289,18 @@ __device__ void stream_body(const StreamArgs& p) {
     walk.compute = list;
   }
   __syncwarp();
+  if (warp < 3 && lane == 0) {
+    // First lines of the CTA's weights, scales and zero points to L2, one array per warp: a prefetch hands no value over, so
+    // it need not wait for the dispatch ahead, and the three address translations pass side by side before the ring begins.
+    const StreamList& list = walk.issue;
+    if (list.row < list.row_end) {
+      const int64_t first = static_cast<int64_t>(list.e) * p.N + list.n0;
+      if (warp == 0) prefetch_l2(p.wq + first * w_pitch, w_pitch);
+      else if (warp == 1) prefetch_l2(p.scales + first * groups, groups * 2);
+      else if (p.zeros) prefetch_l2(p.zeros + first * groups, groups * 2);
+    }
+  }
+  if (!p.offsets && !p.weights_ahead) grid_dependency_wait();
   const uint32_t mask = BF16 ? 0x000f000fu : 0x00f000f0u;
   const uint32_t under = BF16 ? (p.zeros ? 0x43004300u : 0x43084308u) : (p.zeros ? 0x54005400u : 0x54805480u);
   // what the unpacked nibbles stand above their values: of all of them, or without the zero points
