@@ -1766,6 +1766,8 @@ constexpr uint32_t kTilingStageBytes = 64 * (2 * 256 + 16);
 constexpr int kStreamActBytes = 54 * 1024, kStreamSumBytes = 4096;
 constexpr uint32_t kStreamSmemBytes = 16 * (2 * 2048 + 2 * 1024) + 2 * (54 * 1024 + 4096) + 2 * 1025 * 4 + 16 * 304;
 // b200_w4a16_experts_*: 4 activation stages of 32 KiB, 6 raw stages of 8 KiB, 2 staging tiles of 16 KiB, barriers, tables
+// (tiles of 64 rows: 8 of 8 KiB, 12 of 8 KiB)
+constexpr uint32_t kExpertsR64SmemBytes = 1024 + 8 * 8192 + 12 * 8192 + 2 * 16384 + 512 + 2 * 1025 * 4 + 56;
 constexpr uint32_t kExpertsSmemBytes = 1024 + 4 * 32768 + 6 * 8192 + 2 * 16384 + 512 + 2 * 1025 * 4 + 56;
 // b200_expert_route: per expert a next row, an offset and 16 warps' counts, and the rows of 512 slots
 constexpr uint32_t kRouteSmemBytes = 4 * (18 * 1024 + 1 + 512);
@@ -1817,6 +1819,8 @@ const EntryDecl kEntries[] = {
     {"b200_w4a16_stream_bf16_r16", {512, 1, 1}, kStreamSmemBytes},
     {"b200_w4a16_experts_f16", {512, 1, 1}, kExpertsSmemBytes},
     {"b200_w4a16_experts_bf16", {512, 1, 1}, kExpertsSmemBytes},
+    {"b200_w4a16_experts_r64_f16", {768, 1, 1}, kExpertsR64SmemBytes},
+    {"b200_w4a16_experts_r64_bf16", {768, 1, 1}, kExpertsR64SmemBytes},
     {"b200_expert_count", {512, 1, 1}, 0},
     {"b200_expert_route", {512, 1, 1}, kRouteSmemBytes},
     {"b200_expert_combine_f16", {256, 1, 1}, 0},
@@ -2568,11 +2572,12 @@ static bool experts_tensor_fits(const iree_b200_w4a16_experts_params_t* p, const
   return !misaligned(a, 16) && !misaligned(wq, 16) && !misaligned(out, 16) && p->lda % 8 == 0 && p->ldo % 8 == 0 &&
          static_cast<int64_t>(p->experts) * p->N <= INT32_MAX;
 }
-// Rows per expert from which the tensor-core kernel is the faster one.
-constexpr int64_t kExpertsTensorRows = 16;
+// Rows per expert above which the tensor-core kernels are the faster ones (11008 x 4096, 8 experts: 8 rows each 60 us streamed
+// against 66 us, 16 rows 88 against 67), and up to which their tiles of 64 rows are (64 rows 71 us, against 105 with 256).
+constexpr int64_t kExpertsTensorRows = 8, kExpertsR64Rows = 64;
 static int experts_variant(const iree_b200_w4a16_experts_params_t* p, const void* a, const void* wq, const void* out) {
   if (p->variant != IREE_B200_W4A16_EXPERTS_AUTO) return p->variant;
-  return p->rows >= kExpertsTensorRows * p->experts && experts_tensor_fits(p, a, wq, out) ? IREE_B200_W4A16_EXPERTS_TENSOR
+  return p->rows > kExpertsTensorRows * p->experts && experts_tensor_fits(p, a, wq, out) ? IREE_B200_W4A16_EXPERTS_TENSOR
                                                                                            : IREE_B200_W4A16_EXPERTS_STREAM;
 }
 
@@ -2653,14 +2658,17 @@ iree_b200_status_t iree_b200_w4a16_experts_run(iree_b200_context_t* context, con
   if (!tensor)
     return stream_dispatch(context, p.kind, p.rows > 8 * p.experts, a, wq, scales, zeros, offsets, out, p.rows, p.N, p.K,
                            p.group_size, p.lda, p.ldo, p.experts);
-  // at most one part per 256 rows, and one more per expert
-  const int64_t parts = (p.rows + 255) / 256 + (p.rows < p.experts ? p.rows : p.experts);
+  const bool small = p.rows <= kExpertsR64Rows * p.experts;
+  const int64_t tile_rows = small ? 64 : 256;
+  // at most one part per tile's worth of rows, and one more per expert
+  const int64_t parts = (p.rows + tile_rows - 1) / tile_rows + (p.rows < p.experts ? p.rows : p.experts);
   const int64_t tiles = parts * ((p.N + 127) / 128);
   const int sms = usable_sms(context);
   const void* pointers[5] = {scales, zeros, offsets, out, workspace};
   const int32_t constants[6] = {p.rows, p.N, p.K, p.group_size, p.ldo, p.experts};
-  return dispatch_named(context, p.kind == IREE_B200_KIND_F16 ? "b200_w4a16_experts_f16" : "b200_w4a16_experts_bf16", 5,
-                        pointers, 6, constants, static_cast<uint32_t>(tiles < sms ? tiles : sms));
+  const char* name = p.kind == IREE_B200_KIND_F16 ? (small ? "b200_w4a16_experts_r64_f16" : "b200_w4a16_experts_f16")
+                                                  : (small ? "b200_w4a16_experts_r64_bf16" : "b200_w4a16_experts_bf16");
+  return dispatch_named(context, name, 5, pointers, 6, constants, static_cast<uint32_t>(tiles < sms ? tiles : sms));
 }
 
 iree_b200_status_t iree_b200_w4a16_experts(iree_b200_context_t* context, const iree_b200_w4a16_experts_params_t* params,

@@ -24,25 +24,33 @@
 
 namespace b200 {
 
-constexpr int kExWRows = 128;
-constexpr int kExARows = 256;
-constexpr int kExActStages = 4;
-constexpr int kExActStageBytes = kExARows * 128;
-constexpr int kExRawStages = 6;
-constexpr int kExRawStageBytes = kExWRows * 64;
-constexpr int kExAStages = 8;
-constexpr int kExPairStages = kExAStages / 2;
-constexpr int kExAStageColumns = 32;
+constexpr int kExWRows = 128;                                // weight rows per tile = tensor-memory lanes
+constexpr int kExRawStageBytes = kExWRows * 64;              // 128 rows x 128 int4
+constexpr int kExAStageColumns = 32;                         // 64 K as pairs of 16 bits
 constexpr int kExOutRows = 64;
 constexpr int kExOutStageBytes = kExOutRows * kExWRows * 2;
-constexpr int kExThreads = 512;
 constexpr int kExMaxExperts = 1024;
 constexpr int kExBarrierBytes = 512;
 constexpr int kExTableBytes = 2 * (kExMaxExperts + 1) * 4 + 56;
-constexpr int kExSmemBytes = 1024 + kExActStages * kExActStageBytes + kExRawStages * kExRawStageBytes + 2 * kExOutStageBytes +
-                             kExBarrierBytes + kExTableBytes;
-static_assert(kExSmemBytes <= 232448, "per-CTA shared memory limit");
-static_assert(kExARows + kExAStages * kExAStageColumns <= 512, "tensor memory columns");
+
+// Two shapes. Tiles of 256 activation rows: the matrix instructions bound it, two groups of dequant warps keep up. Tiles of 64
+// rows, for experts with few rows: expanding the weights bounds it, four groups, and the memory that activations do not need
+// holds more raw weights on their way.
+template <int AROWS>
+struct Ex {
+  static constexpr bool kSmall = AROWS == 64;
+  static constexpr int kActStages = kSmall ? 8 : 4;
+  static constexpr int kActStageBytes = AROWS * 128;
+  static constexpr int kRawStages = kSmall ? 12 : 6;
+  static constexpr int kPairStages = kSmall ? 6 : 4;         // pairs of K blocks (128 K) expanded in tensor memory
+  static constexpr int kAStages = 2 * kPairStages;
+  static constexpr int kGroups = kSmall ? 4 : 2;             // dequant groups of four warps
+  static constexpr int kThreads = 256 + 128 * kGroups;
+  static constexpr int kSmemBytes = 1024 + kActStages * kActStageBytes + kRawStages * kExRawStageBytes + 2 * kExOutStageBytes +
+                                    kExBarrierBytes + kExTableBytes;
+  static_assert(kSmemBytes <= 232448, "per-CTA shared memory limit");
+  static_assert(AROWS + kAStages * kExAStageColumns <= 512, "tensor memory columns");
+};
 
 struct alignas(128) ExWorkspace {
   uint8_t map_a[128];    // 16-bit [rows, K], 128-byte swizzle, box 64 x 64
@@ -60,6 +68,7 @@ struct ExTile {
 };
 
 // Walks the tiles of one CTA; every role has its own.
+template <int AROWS>
 struct ExWalk {
   const int* first;  // tiles before each expert
   const int* row;    // rows before each expert
@@ -67,7 +76,7 @@ struct ExWalk {
   __device__ ExTile at(int t) {
     while (first[e + 1] <= t) ++e;
     const int local = t - first[e], count = row[e + 1] - row[e];
-    const int parts = (count + kExARows - 1) / kExARows;
+    const int parts = (count + AROWS - 1) / AROWS;
     const int per = ((count + parts - 1) / parts + 15) & ~15;
     const int tn = local / parts, tm = local - tn * parts;
     ExTile x;
@@ -135,25 +144,27 @@ __device__ __forceinline__ void unpack8_minus(uint32_t v, uint32_t offset, uint3
   }
 }
 
-template <bool BF16, bool ZEROS>
+template <int AROWS, bool BF16, bool ZEROS>
 __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t* __restrict__ zeros,
                              const int32_t* __restrict__ offsets, uint16_t* __restrict__ out, ExWorkspace* __restrict__ ws,
                              int rows, int N, int K, int group, int ldo, int experts) {
+  using X = Ex<AROWS>;
+  constexpr int kGroups = X::kGroups;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   uint8_t* smem_gen = smem_raw + (smem_base - smem_u32(smem_raw));
-  const uint32_t raw_base = smem_base + kExActStages * kExActStageBytes;
-  const uint32_t out_base = raw_base + kExRawStages * kExRawStageBytes;
+  const uint32_t raw_base = smem_base + X::kActStages * X::kActStageBytes;
+  const uint32_t out_base = raw_base + X::kRawStages * kExRawStageBytes;
   const uint32_t bars = out_base + 2 * kExOutStageBytes;
   uint8_t* bars_gen = smem_gen + (bars - smem_base);
   int* tile_first = reinterpret_cast<int*>(bars_gen + kExBarrierBytes);
   int* row_first = tile_first + kExMaxExperts + 1;
   auto act_early = [&](int i) { return bars + 8u * i; };  // "the first block of a pair is done with activation stage i"
-  auto raw_full = [&](int i) { return bars + 8u * (kExActStages + i); };
-  auto raw_empty = [&](int i) { return bars + 8u * (kExActStages + kExRawStages + i); };
-  auto a_full = [&](int i) { return bars + 8u * (kExActStages + 2 * kExRawStages + i); };
-  auto a_empty = [&](int i) { return bars + 8u * (kExActStages + 2 * kExRawStages + kExPairStages + i); };
-  constexpr int kNumRingBars = kExActStages + 2 * kExRawStages + 2 * kExPairStages;
+  auto raw_full = [&](int i) { return bars + 8u * (X::kActStages + i); };
+  auto raw_empty = [&](int i) { return bars + 8u * (X::kActStages + X::kRawStages + i); };
+  auto a_full = [&](int i) { return bars + 8u * (X::kActStages + 2 * X::kRawStages + i); };
+  auto a_empty = [&](int i) { return bars + 8u * (X::kActStages + 2 * X::kRawStages + X::kPairStages + i); };
+  constexpr int kNumRingBars = X::kActStages + 2 * X::kRawStages + 2 * X::kPairStages;
   const uint32_t d_full = bars + 8u * kNumRingBars, d_empty = bars + 8u * (kNumRingBars + 1);
   const uint32_t tmem_slot = bars + 8u * (kNumRingBars + 2);
   volatile uint32_t* tmem_slot_ptr = reinterpret_cast<volatile uint32_t*>(bars_gen + 8 * (kNumRingBars + 2));
@@ -166,12 +177,12 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
   const int num_kb = ((K + 127) >> 7) << 1;  // whole pairs of K blocks; TMA fills K behind the end with zeros
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kExActStages; ++i) mbar_init(act_early(i), 1);
-    for (int i = 0; i < kExRawStages; ++i) {
+    for (int i = 0; i < X::kActStages; ++i) mbar_init(act_early(i), 1);
+    for (int i = 0; i < X::kRawStages; ++i) {
       mbar_init(raw_full(i), 1);
       mbar_init(raw_empty(i), 4);
     }
-    for (int i = 0; i < kExPairStages; ++i) {
+    for (int i = 0; i < X::kPairStages; ++i) {
       mbar_init(a_full(i), 5);  // the four warps of a dequant group + the activation tiles' expect_tx
       mbar_init(a_empty(i), 1);
     }
@@ -193,7 +204,7 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
       if (e < experts) {
         lo = min(max(offsets[e], 0), rows);
         const int hi = min(max(offsets[e + 1], lo), rows);
-        need = (hi - lo + kExARows - 1) / kExARows * tiles_n;
+        need = (hi - lo + AROWS - 1) / AROWS * tiles_n;
       }
       int incl = need;
 #pragma unroll
@@ -216,9 +227,9 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = *tmem_slot_ptr;
-  const uint32_t tmem_a = tmem_base + kExARows;
+  const uint32_t tmem_a = tmem_base + AROWS;
   const int num_tiles = tile_first[experts];
-  ExWalk walk = {tile_first, row_first, tiles_n, 0};
+  ExWalk<AROWS> walk = {tile_first, row_first, tiles_n, 0};
 
   // The single-thread roles: the whole warp walks the loop and one elected thread issues, so that the operands of copies and
   // matrix instructions are values which the compiler knows to be uniform and need no move each from a thread's registers
@@ -235,26 +246,31 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
       const int row0 = __shfl_sync(0xffffffffu, x.row0, 0), boxes = __shfl_sync(0xffffffffu, (x.rows + 63) >> 6, 0);
       const uint32_t bytes = 2 * boxes * 64 * 128;
       for (int kb = 0; kb < num_kb; kb += 2, it += 2) {
-        const uint32_t pair = it >> 1, prev = pair - kExActStages / 2;
-        const uint32_t full = a_full(pair % kExPairStages);
-        const uint32_t dst0 = smem_base + (it % kExActStages) * kExActStageBytes;
-        const uint32_t dst1 = smem_base + ((it + 1) % kExActStages) * kExActStageBytes;
+        const uint32_t pair = it >> 1, prev = pair - X::kActStages / 2;
+        const uint32_t full = a_full(pair % X::kPairStages);
+        const uint32_t dst0 = smem_base + (it % X::kActStages) * X::kActStageBytes;
+        const uint32_t dst1 = smem_base + ((it + 1) % X::kActStages) * X::kActStageBytes;
+        // The stages' previous tenants were the blocks of pair - stages / 2; their MMAs' completion is what that pair's "empty"
+        // barrier reports. With four stages of 256 rows that lead would be less than a load takes: the issuer reports the
+        // first block's MMAs on a barrier of its own, and each stage is filled again as soon as its block is done.
         bool waited = true;
-        if (pair >= kExActStages / 2) {
-          const uint32_t prev_block = it - kExActStages;
-          waited = __all_sync(0xffffffffu, mbar_wait(act_early(prev_block % kExActStages), (prev_block / kExActStages) & 1, abort_flag));
+        if (pair >= X::kActStages / 2) {
+          const uint32_t prev_block = it - X::kActStages;
+          if (X::kSmall) waited = __all_sync(0xffffffffu, mbar_wait(a_empty(prev % X::kPairStages), (prev / X::kPairStages) & 1, abort_flag));
+          else waited = __all_sync(0xffffffffu, mbar_wait(act_early(prev_block % X::kActStages), (prev_block / X::kActStages) & 1, abort_flag));
         }
         if (waited) {
           if (leader) {
             mbar_arrive_expect_tx(full, bytes);
             tma_load_3d(dst0, ws->map_a, full, kb * 64, row0, 0);
+            if (X::kSmall) tma_load_3d(dst1, ws->map_a, full, (kb + 1) * 64, row0, 0);
             if (boxes > 1) tma_load_3d(dst0 + 64 * 128, ws->map_a, full, kb * 64, row0 + 64, 0);
             if (boxes > 2) tma_load_3d(dst0 + 128 * 128, ws->map_a, full, kb * 64, row0 + 128, 0);
             if (boxes > 3) tma_load_3d(dst0 + 192 * 128, ws->map_a, full, kb * 64, row0 + 192, 0);
           }
           __syncwarp();
-          if (pair >= kExActStages / 2)
-            waited = __all_sync(0xffffffffu, mbar_wait(a_empty(prev % kExPairStages), (prev / kExPairStages) & 1, abort_flag));
+          if (!X::kSmall && pair >= X::kActStages / 2)
+            waited = __all_sync(0xffffffffu, mbar_wait(a_empty(prev % X::kPairStages), (prev / X::kPairStages) & 1, abort_flag));
         }
         if (!waited) {
           if (leader) {
@@ -264,7 +280,7 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
           ok = false;
           break;
         }
-        if (leader) {
+        if (!X::kSmall && leader) {
           tma_load_3d(dst1, ws->map_a, full, (kb + 1) * 64, row0, 0);
           if (boxes > 1) tma_load_3d(dst1 + 64 * 128, ws->map_a, full, (kb + 1) * 64, row0 + 64, 0);
           if (boxes > 2) tma_load_3d(dst1 + 128 * 128, ws->map_a, full, (kb + 1) * 64, row0 + 128, 0);
@@ -283,8 +299,8 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
       const ExTile x = walk.at(t);
       const int w_row = __shfl_sync(0xffffffffu, x.e * N + x.n0, 0);
       for (int g = 0; g < (num_kb >> 1); ++g, ++raw_it) {
-        const uint32_t rs = raw_it % kExRawStages;
-        if (!__all_sync(0xffffffffu, mbar_wait(raw_empty(rs), ((raw_it / kExRawStages) & 1) ^ 1, abort_flag))) {
+        const uint32_t rs = raw_it % X::kRawStages;
+        if (!__all_sync(0xffffffffu, mbar_wait(raw_empty(rs), ((raw_it / X::kRawStages) & 1) ^ 1, abort_flag))) {
           if (leader) {
             ex_report(ws, kStatusTimeoutEmpty, 0x10000u | raw_it);
             *abort_flag = 1;
@@ -302,9 +318,9 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
   } else if (warp == 1) {
     // -------- MMA issuer -----------------------------------------------------------------------------------
     const uint64_t desc0 = make_smem_desc(smem_base, 16, 1024);
-    constexpr uint32_t kStageUnits = kExActStageBytes >> 4;
+    constexpr uint32_t kStageUnits = X::kActStageBytes >> 4;
     const bool leader = elect_one();
-    const uint32_t d_tmem = __shfl_sync(0xffffffffu, tmem_base, 0), a_tmem = d_tmem + kExARows;
+    const uint32_t d_tmem = __shfl_sync(0xffffffffu, tmem_base, 0), a_tmem = d_tmem + AROWS;
     uint32_t it = 0, local_tile = 0;
     bool ok = true;
     for (int t = blockIdx.x; t < tiles && ok; t += gridDim.x, ++local_tile) {
@@ -320,8 +336,8 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
       }
       tc_fence_after_sync();
       for (int kb = 0; kb < num_kb; kb += 2, it += 2) {
-        const uint32_t pair = it >> 1, ps = pair % kExPairStages;
-        if (!__all_sync(0xffffffffu, mbar_wait(a_full(ps), (pair / kExPairStages) & 1, abort_flag))) {
+        const uint32_t pair = it >> 1, ps = pair % X::kPairStages;
+        if (!__all_sync(0xffffffffu, mbar_wait(a_full(ps), (pair / X::kPairStages) & 1, abort_flag))) {
           if (leader) {
             ex_report(ws, kStatusTimeoutDequant, it);
             *abort_flag = 1;
@@ -330,15 +346,15 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
           break;
         }
         tc_fence_after_sync();
-        const uint64_t b0 = desc0 + (it % kExActStages) * kStageUnits, b1 = desc0 + ((it + 1) % kExActStages) * kStageUnits;
-        const uint32_t a0 = a_tmem + (it % kExAStages) * kExAStageColumns, a1 = a_tmem + ((it + 1) % kExAStages) * kExAStageColumns;
+        const uint64_t b0 = desc0 + (it % X::kActStages) * kStageUnits, b1 = desc0 + ((it + 1) % X::kActStages) * kStageUnits;
+        const uint32_t a0 = a_tmem + (it % X::kAStages) * kExAStageColumns, a1 = a_tmem + ((it + 1) % X::kAStages) * kExAStageColumns;
         if (leader) {
           if (kb == 0) mma_f16_ts_first(d_tmem, a0, b0, idesc);
           else mma_f16_ts_more(d_tmem, a0, b0, idesc);
           mma_f16_ts_more(d_tmem, a0 + 8, b0 + 2, idesc);
           mma_f16_ts_more(d_tmem, a0 + 16, b0 + 4, idesc);
           mma_f16_ts_more(d_tmem, a0 + 24, b0 + 6, idesc);
-          tc_commit(act_early(it % kExActStages));
+          if (!X::kSmall) tc_commit(act_early(it % X::kActStages));
           mma_f16_ts_more(d_tmem, a1, b1, idesc);
           mma_f16_ts_more(d_tmem, a1 + 8, b1 + 2, idesc);
           mma_f16_ts_more(d_tmem, a1 + 16, b1 + 4, idesc);
@@ -424,7 +440,7 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
     // -------- dequant: raw int4 (64-byte swizzled rows) -> 64 columns of this thread's TMEM lane, a pair of K blocks at a time --
     const int td = threadIdx.x - 256;
     const int r = td & 127;   // weight row of the tile = TMEM lane
-    const uint32_t grp = td >> 7;  // pairs grp, grp + 2, ... of the CTA's sequence
+    const uint32_t grp = td >> 7;  // pairs grp, grp + groups, ... of the CTA's sequence
     const int groups = K / group;
     // Scale groups that a pair (128 K) holds: 1, 2 or 4, aligned with it; or any (a group of 96), one per 32 K.
     const int per_pair = group % 128 == 0 ? 1 : group == 64 ? 2 : 4;
@@ -487,11 +503,11 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
           }
         }
       };
-      int p = (grp - pair_base) & 1;
+      int p = (grp - pair_base) & (kGroups - 1);
       if (p < pairs) fetch(p);
-      for (; p < pairs; p += 2) {
-        const uint32_t pair = pair_base + p, ps = pair % kExPairStages;
-        const int rs = pair % kExRawStages;
+      for (; p < pairs; p += kGroups) {
+        const uint32_t pair = pair_base + p, ps = pair % X::kPairStages;
+        const int rs = pair % X::kRawStages;
         uint32_t s2[4], off2[4], z2[4];
         bool whole = true;
 #pragma unroll
@@ -507,9 +523,9 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
             z2[c] = 0;
           }
         }
-        if (p + 2 < pairs) fetch(p + 2);
+        if (p + kGroups < pairs) fetch(p + kGroups);
         const bool fast = !ZEROS || __all_sync(0xffffffffu, whole);
-        if (!__all_sync(0xffffffffu, mbar_wait(raw_full(rs), (pair / kExRawStages) & 1, abort_flag))) {
+        if (!__all_sync(0xffffffffu, mbar_wait(raw_full(rs), (pair / X::kRawStages) & 1, abort_flag))) {
           if (lane == 0) {
             ex_report(ws, kStatusTimeoutFull, 0x10000u | pair);
             *abort_flag = 1;
@@ -517,7 +533,7 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
           ok = false;
           break;
         }
-        if (!__all_sync(0xffffffffu, mbar_wait(a_empty(ps), ((pair / kExPairStages) & 1) ^ 1, abort_flag))) {
+        if (!__all_sync(0xffffffffu, mbar_wait(a_empty(ps), ((pair / X::kPairStages) & 1) ^ 1, abort_flag))) {
           if (lane == 0) {
             ex_report(ws, kStatusTimeoutEmpty, 0x20000u | pair);
             *abort_flag = 1;
@@ -554,7 +570,7 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
               }
             }
           }
-          tmem_st_32x32(tmem_a + lane_base + ((pair * 2 + h) % kExAStages) * kExAStageColumns, v);
+          tmem_st_32x32(tmem_a + lane_base + ((pair * 2 + h) % X::kAStages) * kExAStageColumns, v);
         }
         tc_wait_st();
         tc_fence_before_sync();
@@ -583,14 +599,16 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
 }  // namespace b200
 
 // Bindings: scales, zero points (NULL: signed weights), row offsets, result, workspace.
-#define B200_W4A16_EXPERTS(NAME, BF16)                                                                                     \
-  extern "C" __global__ void __launch_bounds__(b200::kExThreads, 1)                                                        \
+#define B200_W4A16_EXPERTS(NAME, AROWS, BF16)                                                                              \
+  extern "C" __global__ void __launch_bounds__(b200::Ex<AROWS>::kThreads, 1)                                               \
       NAME(const uint16_t* scales, const uint16_t* zeros, const int32_t* offsets, uint16_t* out, void* ws, int rows, int N,  \
            int K, int group, int ldo, int experts) {                                                                       \
     b200::ExWorkspace* w = reinterpret_cast<b200::ExWorkspace*>(ws);                                                       \
-    if (zeros) b200::experts_body<BF16, true>(scales, zeros, offsets, out, w, rows, N, K, group, ldo, experts);            \
-    else b200::experts_body<BF16, false>(scales, zeros, offsets, out, w, rows, N, K, group, ldo, experts);                 \
+    if (zeros) b200::experts_body<AROWS, BF16, true>(scales, zeros, offsets, out, w, rows, N, K, group, ldo, experts);     \
+    else b200::experts_body<AROWS, BF16, false>(scales, zeros, offsets, out, w, rows, N, K, group, ldo, experts);          \
   }
-B200_W4A16_EXPERTS(b200_w4a16_experts_f16, false)
-B200_W4A16_EXPERTS(b200_w4a16_experts_bf16, true)
+B200_W4A16_EXPERTS(b200_w4a16_experts_f16, 256, false)
+B200_W4A16_EXPERTS(b200_w4a16_experts_bf16, 256, true)
+B200_W4A16_EXPERTS(b200_w4a16_experts_r64_f16, 64, false)
+B200_W4A16_EXPERTS(b200_w4a16_experts_r64_bf16, 64, true)
 #undef B200_W4A16_EXPERTS
