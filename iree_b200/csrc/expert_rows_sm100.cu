@@ -10,8 +10,8 @@
 // (8-byte and single elements otherwise); sums are f32, in slot order, rounded once. No atomics decide an order.
 //
 // The sort counts. One CTA owns a run of tokens; what it has to know of the rest is how many slots go to each expert before
-// its run and in all. Up to kRouteSingle slots every CTA counts all of them itself, one launch; above that a first launch
-// leaves one histogram per run and every CTA adds them up. Ranks inside a run come from warp votes.
+// its run and in all. Up to 8192 slots every CTA counts all of them itself, one launch; above that a first launch leaves one
+// histogram per run and a second one sums them along the runs. Ranks inside a run come from warp votes.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
@@ -23,7 +23,6 @@ namespace b200 {
 constexpr int kRouteThreads = 512;
 constexpr int kRouteWarps = kRouteThreads / 32;
 constexpr int kRouteMaxExperts = 1024;
-constexpr int kRouteMaxSlots = 256;
 constexpr int kRouteRun = kRouteThreads;  // slots of a run that are ranked at a time: one per thread
 
 template <int V>
@@ -64,7 +63,7 @@ __device__ void move_rows(const uint16_t* __restrict__ x, uint16_t* __restrict__
   using P = typename Piece<V>::type;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int width = (d1 - d0) / V;
-  constexpr int U = 4;
+  constexpr int U = 8;
   const int strips = (width + 32 * U - 1) / (32 * U);
   for (int w = warp; w < tokens * strips; w += kRouteWarps) {
     const int t = w / strips, s = w - t * strips;
@@ -107,16 +106,56 @@ extern "C" __global__ void __launch_bounds__(b200::kRouteThreads)
   for (int e = threadIdx.x; e < experts; e += kRouteThreads) counts[static_cast<int64_t>(blockIdx.x) * experts + e] = hist[e];
 }
 
-// Grid: runs of tokens x column parts. counts: of b200_expert_count, or NULL (every CTA counts all ids).
+// The runs' histograms become, in place, the slots of each expert in the runs before; totals[expert]: in all runs. A CTA owns
+// 32 experts (a lane each), its 16 warps equal parts of the runs.
 extern "C" __global__ void __launch_bounds__(b200::kRouteThreads)
-    b200_expert_route(const int32_t* ids, const int32_t* counts, const uint16_t* x, int32_t* offsets, int32_t* position,
+    b200_expert_scan(int32_t* counts, int32_t* totals, int runs, int experts) {
+  __shared__ int part_sum[kRouteWarps][32];
+  grid_launch_dependents();
+  grid_dependency_wait();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e = blockIdx.x * 32 + lane;
+  const int per = (runs + kRouteWarps - 1) / kRouteWarps, lo = warp * per, hi = min(lo + per, runs);
+  constexpr int kBatch = 20;  // loads in flight per thread: all of a part up to 2 x 148 runs
+  int sum = 0;
+  for (int r0 = lo; r0 < hi; r0 += kBatch) {
+    int c[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) c[i] = r0 + i < hi && e < experts ? counts[static_cast<int64_t>(r0 + i) * experts + e] : 0;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) sum += c[i];
+  }
+  part_sum[warp][lane] = sum;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < kRouteWarps; ++w) {
+    if (w < warp) before += part_sum[w][lane];
+    all += part_sum[w][lane];
+  }
+  for (int r0 = lo; r0 < hi; r0 += kBatch) {
+    int c[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) c[i] = r0 + i < hi && e < experts ? counts[static_cast<int64_t>(r0 + i) * experts + e] : 0;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (r0 + i < hi && e < experts) counts[static_cast<int64_t>(r0 + i) * experts + e] = before;
+      before += c[i];
+    }
+  }
+  if (warp == 0 && e < experts) totals[e] = all;
+}
+
+// Grid: runs of tokens x column parts. counts, totals: of b200_expert_scan, or NULL (every CTA counts all ids).
+extern "C" __global__ void __launch_bounds__(b200::kRouteThreads)
+    b200_expert_route(const int32_t* ids, const int32_t* counts, const int32_t* totals, const uint16_t* x, int32_t* offsets, int32_t* position,
                       int32_t* order, uint16_t* rows, int tokens, int slots, int experts, int first, int run, int width,
                       int ldx, int ldr, int part_width, int vec) {
   extern __shared__ int shared[];
-  int* next = shared;                      // the run's next row of each expert
-  int* total = next + experts;             // slots per expert, then offsets
-  int* warp_count = total + experts + 1;   // [warp][expert]
-  int* where = warp_count + kRouteWarps * experts;  // rows of the slots of one piece of the run
+  int* next = shared;                  // the run's next row of each expert
+  int* base = next + experts;          // the same at the start of the piece that is ranked
+  int* total = base + experts;         // slots per expert, then offsets
+  int* where = total + experts + 1;    // rows of the slots of one piece of the run
+  uint16_t* warp_count = reinterpret_cast<uint16_t*>(where + kRouteRun);  // [warp][expert], then slots of the warps before
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   for (int e = tid; e < experts; e += kRouteThreads) next[e] = total[e] = 0;
   grid_launch_dependents();
@@ -125,29 +164,22 @@ extern "C" __global__ void __launch_bounds__(b200::kRouteThreads)
   const int64_t all = static_cast<int64_t>(tokens) * slots;
   const int64_t t_lo = static_cast<int64_t>(blockIdx.x) * run, t_hi = min(t_lo + run, static_cast<int64_t>(tokens));
   if (counts) {
-    // threads along experts first, then along runs: (experts rounded up to a warp) x parts
-    const int cols = (experts + 31) & ~31;
-    const int parts = max(1, kRouteThreads / cols);
-    for (int i = tid; i < cols * parts; i += kRouteThreads) {
-      const int e = i % cols, part = i / cols;
-      if (e < experts) {
-        int sum = 0, before = 0;
-#pragma unroll 8
-        for (int r = part; r < static_cast<int>(gridDim.x); r += parts) {
-          const int c = counts[static_cast<int64_t>(r) * experts + e];
-          sum += c;
-          if (r < static_cast<int>(blockIdx.x)) before += c;
-        }
-        if (sum) atomicAdd(&total[e], sum);
-        if (before) atomicAdd(&next[e], before);
-      }
+    for (int e = tid; e < experts; e += kRouteThreads) {
+      total[e] = totals[e];
+      next[e] = counts[static_cast<int64_t>(blockIdx.x) * experts + e];
     }
   } else {
-    for (int64_t i = tid; i < all; i += kRouteThreads) {
-      const int e = local_expert(ids[i], first, experts);
-      if (e >= 0) {
-        atomicAdd(&total[e], 1);
-        if (i < t_lo * slots) atomicAdd(&next[e], 1);
+    constexpr int kBatch = 8;  // ids loaded at a time
+    for (int64_t i0 = tid; i0 < all; i0 += kRouteThreads * kBatch) {
+      int id[kBatch];
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) id[i] = i0 + i * kRouteThreads < all ? local_expert(ids[i0 + i * kRouteThreads], first, experts) : -1;
+#pragma unroll
+      for (int i = 0; i < kBatch; ++i) {
+        if (id[i] >= 0) {
+          atomicAdd(&total[id[i]], 1);
+          if (i0 + i * kRouteThreads < t_lo * slots) atomicAdd(&next[id[i]], 1);
+        }
       }
     }
   }
@@ -189,20 +221,22 @@ extern "C" __global__ void __launch_bounds__(b200::kRouteThreads)
     const int e = tid < n ? local_expert(ids[t0 * slots + tid], first, experts) : -1;
     const unsigned peers = __match_any_sync(0xffffffffu, e);
     const int rank = __popc(peers & ((1u << lane) - 1u));
-    if (e >= 0 && rank == 0) warp_count[warp * experts + e] = __popc(peers);
+    if (e >= 0 && rank == 0) warp_count[warp * experts + e] = static_cast<uint16_t>(__popc(peers));
     __syncthreads();
-    for (int x_e = tid; x_e < experts; x_e += kRouteThreads) {  // rows of each warp's first slot of the expert
-      int at = next[x_e];
+    for (int x_e = tid; x_e < experts; x_e += kRouteThreads) {  // slots of the expert in the warps before each one
+      int at = 0;
+#pragma unroll
       for (int w = 0; w < kRouteWarps; ++w) {
         const int c = warp_count[w * experts + x_e];
-        warp_count[w * experts + x_e] = at;
+        warp_count[w * experts + x_e] = static_cast<uint16_t>(at);
         at += c;
       }
-      next[x_e] = at;
+      base[x_e] = next[x_e];
+      next[x_e] += at;
     }
     __syncthreads();
     if (tid < n) {
-      const int pos = e >= 0 ? warp_count[warp * experts + e] + rank : -1;
+      const int pos = e >= 0 ? base[e] + warp_count[warp * experts + e] + rank : -1;
       where[tid] = pos;
       if (writes) {
         position[t0 * slots + tid] = pos;
@@ -223,8 +257,10 @@ namespace b200 {
 constexpr int kCombineThreads = 256;
 constexpr int kCombineWarps = kCombineThreads / 32;
 
-// A warp owns a strip of 32 * V * U columns of one token and adds the slots' rows in order.
-template <bool BF16, int V, int U>
+// A warp owns a strip of 32 * V * U columns of one token and adds the slots' rows in order. J > 1: J slots' places first,
+// then all their pieces (8-byte pieces need the more of them on their way: 4095 x 4 rows of 2044 in 15.7 us, 20.4 with J = 1,
+// U = 2; 16-byte pieces lose the warps that the registers cost: 8192 x 2 rows of 4096 in 34.5 us against 40.4 with J = 2).
+template <bool BF16, int V, int U, int J>
 __device__ void combine_body(const uint16_t* __restrict__ rows, const float* __restrict__ weights,
                              const int32_t* __restrict__ position, uint16_t* __restrict__ out, int tokens, int slots,
                              int width, int64_t ldr, int64_t ldo, int row_count) {
@@ -240,22 +276,54 @@ __device__ void combine_body(const uint16_t* __restrict__ rows, const float* __r
   for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int i = 0; i < V; ++i) acc[u][i] = 0.f;
-#pragma unroll 4
-  for (int j = 0; j < slots; ++j) {
-    const int pos = position[t * slots + j];
-    if (static_cast<unsigned>(pos) >= static_cast<unsigned>(row_count)) continue;
-    const float weight = weights ? weights[t * slots + j] : 1.f;
-    const P* src = reinterpret_cast<const P*>(rows + pos * ldr);
-    PieceValues<V> v[U];
+  if constexpr (J > 1) {
+    for (int j0 = 0; j0 < slots; j0 += J) {
+      int pos[J];
+      float weight[J];
 #pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (c0 + 32 * u < pieces) v[u].piece = src[c0 + 32 * u];
-#pragma unroll
-    for (int u = 0; u < U; ++u)
-      if (c0 + 32 * u < pieces) {
-#pragma unroll
-        for (int i = 0; i < V; ++i) acc[u][i] = fmaf(weight, to_float<BF16>(v[u].e[i]), acc[u][i]);
+      for (int j = 0; j < J; ++j) {
+        pos[j] = j0 + j < slots ? position[t * slots + j0 + j] : -1;
+        if (static_cast<unsigned>(pos[j]) >= static_cast<unsigned>(row_count)) pos[j] = -1;
+        weight[j] = weights && j0 + j < slots ? weights[t * slots + j0 + j] : 1.f;
       }
+      PieceValues<V> v[J][U];
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        const P* src = reinterpret_cast<const P*>(rows + pos[j] * ldr);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (pos[j] >= 0 && c0 + 32 * u < pieces) v[j][u].piece = src[c0 + 32 * u];
+      }
+#pragma unroll
+      for (int j = 0; j < J; ++j) {
+        if (pos[j] >= 0) {
+#pragma unroll
+          for (int u = 0; u < U; ++u)
+            if (c0 + 32 * u < pieces) {
+#pragma unroll
+              for (int i = 0; i < V; ++i) acc[u][i] = fmaf(weight[j], to_float<BF16>(v[j][u].e[i]), acc[u][i]);
+            }
+        }
+      }
+    }
+  } else {
+#pragma unroll 4
+    for (int j = 0; j < slots; ++j) {
+      const int pos = position[t * slots + j];
+      if (static_cast<unsigned>(pos) >= static_cast<unsigned>(row_count)) continue;
+      const float weight = weights ? weights[t * slots + j] : 1.f;
+      const P* src = reinterpret_cast<const P*>(rows + pos * ldr);
+      PieceValues<V> v[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (c0 + 32 * u < pieces) v[u].piece = src[c0 + 32 * u];
+#pragma unroll
+      for (int u = 0; u < U; ++u)
+        if (c0 + 32 * u < pieces) {
+#pragma unroll
+          for (int i = 0; i < V; ++i) acc[u][i] = fmaf(weight, to_float<BF16>(v[u].e[i]), acc[u][i]);
+        }
+    }
   }
   P* dst = reinterpret_cast<P*>(out + t * ldo);
 #pragma unroll
@@ -316,16 +384,23 @@ __device__ void combine_backward_body(const uint16_t* __restrict__ dout, const u
 }  // namespace b200
 
 #define B200_EXPERT_COMBINE(SUFFIX, BF16)                                                                                  \
-  extern "C" __global__ void __launch_bounds__(b200::kCombineThreads)                                                      \
+  extern "C" __global__ void __launch_bounds__(b200::kCombineThreads, 6)                                                   \
       b200_expert_combine_##SUFFIX(const uint16_t* rows, const float* weights, const int32_t* position, uint16_t* out,     \
-                                   int tokens, int slots, int width, int ldr, int ldo, int row_count, int vec) {           \
+                                   int tokens, int slots, int width, int ldr, int ldo, int row_count) {                    \
     grid_launch_dependents();                                                                                              \
     grid_dependency_wait();                                                                                                \
-    if (vec == 8) combine_body<BF16, 8, 2>(rows, weights, position, out, tokens, slots, width, ldr, ldo, row_count);       \
-    else if (vec == 4) combine_body<BF16, 4, 2>(rows, weights, position, out, tokens, slots, width, ldr, ldo, row_count);  \
-    else combine_body<BF16, 1, 2>(rows, weights, position, out, tokens, slots, width, ldr, ldo, row_count);                \
+    combine_body<BF16, 8, 2, 1>(rows, weights, position, out, tokens, slots, width, ldr, ldo, row_count);                     \
   }                                                                                                                        \
   extern "C" __global__ void __launch_bounds__(b200::kCombineThreads)                                                      \
+      b200_expert_combine_narrow_##SUFFIX(const uint16_t* rows, const float* weights, const int32_t* position,             \
+                                          uint16_t* out, int tokens, int slots, int width, int ldr, int ldo,               \
+                                          int row_count, int vec) {                                                        \
+    grid_launch_dependents();                                                                                              \
+    grid_dependency_wait();                                                                                                \
+    if (vec == 4) combine_body<BF16, 4, 4, 2>(rows, weights, position, out, tokens, slots, width, ldr, ldo, row_count);       \
+    else combine_body<BF16, 1, 2, 4>(rows, weights, position, out, tokens, slots, width, ldr, ldo, row_count);                \
+  }                                                                                                                        \
+  extern "C" __global__ void __launch_bounds__(b200::kCombineThreads, 6)                                                   \
       b200_expert_combine_backward_##SUFFIX(const uint16_t* dout, const uint16_t* rows, const float* weights,              \
                                             const int32_t* position, uint16_t* drows, float* dweights, int tokens,         \
                                             int slots, int width, int ldo, int ldr, int row_count, int vec) {              \

@@ -1769,8 +1769,8 @@ constexpr uint32_t kStreamSmemBytes = 16 * (2 * 2048 + 2 * 1024) + 2 * (54 * 102
 // (tiles of 64 rows: 8 of 8 KiB, 12 of 8 KiB)
 constexpr uint32_t kExpertsR64SmemBytes = 1024 + 8 * 8192 + 12 * 8192 + 2 * 16384 + 512 + 2 * 1025 * 4 + 56;
 constexpr uint32_t kExpertsSmemBytes = 1024 + 4 * 32768 + 6 * 8192 + 2 * 16384 + 512 + 2 * 1025 * 4 + 56;
-// b200_expert_route: per expert a next row, an offset and 16 warps' counts, and the rows of 512 slots
-constexpr uint32_t kRouteSmemBytes = 4 * (18 * 1024 + 1 + 512);
+// b200_expert_route: per expert a next row, its start, an offset and 16 warps' counts, and the rows of 512 slots
+constexpr uint32_t kRouteSmemBytes = 4 * (3 * 1024 + 1 + 512) + 2 * 16 * 1024;
 constexpr int kMaxExperts = 1024;
 constexpr int kMaxSlots = 256;
 constexpr int kMaxStreamK = 1 << 20;  // the kernels divide K / 32 by group / 32 through a 32-bit reciprocal
@@ -1822,9 +1822,12 @@ const EntryDecl kEntries[] = {
     {"b200_w4a16_experts_r64_f16", {768, 1, 1}, kExpertsR64SmemBytes},
     {"b200_w4a16_experts_r64_bf16", {768, 1, 1}, kExpertsR64SmemBytes},
     {"b200_expert_count", {512, 1, 1}, 0},
+    {"b200_expert_scan", {512, 1, 1}, 0},
     {"b200_expert_route", {512, 1, 1}, kRouteSmemBytes},
     {"b200_expert_combine_f16", {256, 1, 1}, 0},
     {"b200_expert_combine_bf16", {256, 1, 1}, 0},
+    {"b200_expert_combine_narrow_f16", {256, 1, 1}, 0},
+    {"b200_expert_combine_narrow_bf16", {256, 1, 1}, 0},
     {"b200_expert_combine_backward_f16", {256, 1, 1}, 0},
     {"b200_expert_combine_backward_bf16", {256, 1, 1}, 0},
     {"b200_mmt4d_s8s8s32", {512, 1, 1}, kMmt4dSmemBytes},
@@ -2730,8 +2733,8 @@ static void route_grid(const iree_b200_expert_rows_params_t* p, int sms, int* ru
 size_t iree_b200_expert_dispatch_workspace_bytes(const iree_b200_expert_rows_params_t* params) {
   if (rows_validate(params) != IREE_B200_STATUS_OK) return 0;
   if (static_cast<int64_t>(params->tokens) * params->slots <= kRouteSingleSlots) return 0;
-  // one histogram per run; at most 2 x 148 runs on any device this library drives, whatever SMs are reserved
-  return static_cast<size_t>(2 * 148) * params->experts * sizeof(int32_t);
+  // one histogram per run and their sum; at most 2 x 148 runs on any device this library drives, whatever SMs are reserved
+  return static_cast<size_t>(2 * 148 + 1) * params->experts * sizeof(int32_t);
 }
 
 iree_b200_status_t iree_b200_expert_dispatch(iree_b200_context_t* context, const iree_b200_expert_rows_params_t* params,
@@ -2750,15 +2753,19 @@ iree_b200_status_t iree_b200_expert_dispatch(iree_b200_context_t* context, const
   if (sms > 148) sms = 148;
   int run, runs, part_width, parts;
   route_grid(&p, sms, &run, &runs, &part_width, &parts);
+  void* totals = counted ? static_cast<int32_t*>(workspace) + static_cast<size_t>(runs) * p.experts : nullptr;
   if (counted) {
     const void* pointers[2] = {expert_ids, workspace};
     const int32_t constants[5] = {p.tokens, p.slots, p.experts, p.first_expert, run};
     B200_RETURN_IF_ERROR(dispatch_named(context, "b200_expert_count", 2, pointers, 5, constants, runs));
+    const void* scan_pointers[2] = {workspace, totals};
+    const int32_t scan_constants[2] = {runs, p.experts};
+    B200_RETURN_IF_ERROR(dispatch_named(context, "b200_expert_scan", 2, scan_pointers, 2, scan_constants, (p.experts + 31) / 32));
   }
-  const void* pointers[7] = {expert_ids, counted ? workspace : nullptr, x, offsets, position, order, rows};
+  const void* pointers[8] = {expert_ids, counted ? workspace : nullptr, counted ? totals : nullptr, x, offsets, position, order, rows};
   const int32_t constants[10] = {p.tokens, p.slots, p.experts, p.first_expert, run, p.width, p.token_pitch, p.row_pitch,
                                  part_width, rows_vector(&p, x, rows, nullptr)};
-  return dispatch_named(context, "b200_expert_route", 7, pointers, 10, constants, runs, parts);
+  return dispatch_named(context, "b200_expert_route", 8, pointers, 10, constants, runs, parts);
 }
 
 static iree_b200_status_t combine_dispatch(iree_b200_context_t* context, const iree_b200_expert_rows_params_t& p,
@@ -2770,11 +2777,15 @@ static iree_b200_status_t combine_dispatch(iree_b200_context_t* context, const i
   if (!context) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "context is NULL");
   if (empty) return IREE_B200_STATUS_OK;
   const int vec = rows_vector(&p, out, rows, nullptr);
-  const int64_t strips = (p.width / vec + 63) / 64;
+  const int strip = vec == 4 ? 128 : 64;  // pieces of a warp's strip
+  const int64_t strips = (p.width / vec + strip - 1) / strip;
   const void* pointers[4] = {rows, weights, position, out};
   const int32_t constants[7] = {p.tokens, p.slots, p.width, p.row_pitch, p.token_pitch, p.tokens * p.slots, vec};
-  return dispatch_named(context, p.kind == IREE_B200_KIND_F16 ? "b200_expert_combine_f16" : "b200_expert_combine_bf16", 4,
-                        pointers, 7, constants, static_cast<uint32_t>((p.tokens * strips + 7) / 8));
+  const bool f16 = p.kind == IREE_B200_KIND_F16;
+  const char* name = vec == 8 ? (f16 ? "b200_expert_combine_f16" : "b200_expert_combine_bf16")
+                              : (f16 ? "b200_expert_combine_narrow_f16" : "b200_expert_combine_narrow_bf16");
+  return dispatch_named(context, name, 4, pointers, vec == 8 ? 6 : 7, constants,
+                        static_cast<uint32_t>((p.tokens * strips + 7) / 8));
 }
 
 iree_b200_status_t iree_b200_expert_combine(iree_b200_context_t* context, const iree_b200_expert_rows_params_t* params,
