@@ -653,8 +653,11 @@ typedef struct {
   int32_t lda, ldo;
   int32_t variant; /* IREE_B200_W4A16_EXPERTS_* */
 } iree_b200_w4a16_experts_params_t;
-/* prepare() picks the variant and writes what it needs into the workspace (128-byte aligned, the given size, not shared
- * between dispatches in flight); run() dispatches and may be repeated while operands stay in place. */
+/* prepare() picks the variant (TENSOR above 8 rows per expert, where its copies reach the operands) and writes what it needs
+ * into the workspace: 128-byte aligned, the given size, not shared between dispatches in flight; for TENSOR this is a copy,
+ * which a graph that is being recorded refuses (FAILED_PRECONDITION). run() dispatches and may be repeated, and recorded, while
+ * operands stay in place; with other operands or sizes than prepare() saw, TENSOR computes nothing and
+ * iree_b200_workspace_status reports INVALID_ARGUMENT. */
 size_t iree_b200_w4a16_experts_workspace_bytes(const iree_b200_w4a16_experts_params_t* params);
 iree_b200_status_t iree_b200_w4a16_experts_prepare(iree_b200_context_t* context,
                                                    const iree_b200_w4a16_experts_params_t* params, const void* a,

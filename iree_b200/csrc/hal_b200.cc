@@ -1772,6 +1772,7 @@ constexpr uint32_t kExpertsSmemBytes = 1024 + 4 * 32768 + 6 * 8192 + 2 * 16384 +
 // b200_expert_route: per expert a next row, its start, an offset and 16 warps' counts, and the rows of 512 slots
 constexpr uint32_t kRouteSmemBytes = 4 * (3 * 1024 + 1 + 512) + 2 * 16 * 1024;
 constexpr int kMaxExperts = 1024;
+constexpr uint32_t kExpertsNoteMagic = 0x45585034u;
 constexpr int kMaxSlots = 256;
 constexpr int kMaxStreamK = 1 << 20;  // the kernels divide K / 32 by group / 32 through a 32-bit reciprocal
 // Up to this many slots every CTA of the routing kernel counts all of them itself (one launch).
@@ -1865,6 +1866,8 @@ struct iree_b200_context_t {
   bool dispatch_overlap = false;
   // SMs the operator entry points leave free (for collectives that run beside the dispatches)
   int reserved_sms = 0;
+  // ordinals of the exports that dispatch_named has looked up, by the address of their (literal) names
+  std::vector<std::pair<const char*, int32_t>> ordinals;
 };
 
 namespace {
@@ -2482,8 +2485,14 @@ static bool misaligned(const void* p, uintptr_t bytes) { return (reinterpret_cas
 static iree_b200_status_t dispatch_named(iree_b200_context_t* context, const char* name, int binding_count,
                                          const void* const* pointers, int constant_count, const int32_t* constants,
                                          uint32_t grid_x, uint32_t grid_y = 1) {
-  const int32_t ord = iree_hal_b200_executable_lookup(context->executable, name);
-  if (ord < 0) return fail(IREE_B200_STATUS_NOT_FOUND, "export %s missing from the executable", name);
+  int32_t ord = -1;
+  for (const auto& known : context->ordinals)
+    if (known.first == name) ord = known.second;
+  if (ord < 0) {
+    ord = iree_hal_b200_executable_lookup(context->executable, name);
+    if (ord < 0) return fail(IREE_B200_STATUS_NOT_FOUND, "export %s missing from the executable", name);
+    context->ordinals.emplace_back(name, ord);
+  }
   auto* cb = context->command_buffer;
   iree_hal_b200_descriptor_set_binding_t bindings[IREE_HAL_B200_MAX_DESCRIPTOR_SET_BINDING_COUNT];
   for (int i = 0; i < binding_count; ++i) bindings[i] = {static_cast<uint32_t>(i), const_cast<void*>(pointers[i])};
@@ -2635,6 +2644,14 @@ iree_b200_status_t iree_b200_w4a16_experts_prepare(iree_b200_context_t* context,
   B200_RETURN_IF_ERROR(encode_map(CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, CU_TENSOR_MAP_SWIZZLE_64B, 64, wq, p.K / 2,
                                   static_cast<uint32_t>(p.experts) * p.N, 1, 64, 128, host + 128));
   B200_RETURN_IF_ERROR(encode_output_map(out, p.N, p.rows, static_cast<uint64_t>(p.ldo) * 2, host + 256));
+  // what the maps are for (words 18.. of the status words): the kernel computes nothing through a workspace without this note
+  const uint64_t addresses[3] = {reinterpret_cast<uint64_t>(a), reinterpret_cast<uint64_t>(wq), reinterpret_cast<uint64_t>(out)};
+  const uint32_t note[8] = {kExpertsNoteMagic, p.kind == IREE_B200_KIND_BF16, static_cast<uint32_t>(p.rows),
+                            static_cast<uint32_t>(p.N), static_cast<uint32_t>(p.K), static_cast<uint32_t>(p.lda),
+                            static_cast<uint32_t>(p.ldo), static_cast<uint32_t>(p.experts)};
+  memcpy(host + 384 + 18 * 4, note, sizeof note);
+  memcpy(host + 384 + 26 * 4, addresses, sizeof addresses);
+  context->command_buffer->barrier_pending = true;  // a kernel may not be launched early behind a copy
   return iree_hal_b200_transfer_h2d(context->device, host, workspace, sizeof host);
 }
 
@@ -2667,11 +2684,11 @@ iree_b200_status_t iree_b200_w4a16_experts_run(iree_b200_context_t* context, con
   const int64_t parts = (p.rows + tile_rows - 1) / tile_rows + (p.rows < p.experts ? p.rows : p.experts);
   const int64_t tiles = parts * ((p.N + 127) / 128);
   const int sms = usable_sms(context);
-  const void* pointers[5] = {scales, zeros, offsets, out, workspace};
-  const int32_t constants[6] = {p.rows, p.N, p.K, p.group_size, p.ldo, p.experts};
+  const void* pointers[7] = {scales, zeros, offsets, out, a, wq, workspace};
+  const int32_t constants[7] = {p.rows, p.N, p.K, p.group_size, p.lda, p.ldo, p.experts};
   const char* name = p.kind == IREE_B200_KIND_F16 ? (small ? "b200_w4a16_experts_r64_f16" : "b200_w4a16_experts_f16")
                                                   : (small ? "b200_w4a16_experts_r64_bf16" : "b200_w4a16_experts_bf16");
-  return dispatch_named(context, name, 5, pointers, 6, constants, static_cast<uint32_t>(tiles < sms ? tiles : sms));
+  return dispatch_named(context, name, 7, pointers, 7, constants, static_cast<uint32_t>(tiles < sms ? tiles : sms));
 }
 
 iree_b200_status_t iree_b200_w4a16_experts(iree_b200_context_t* context, const iree_b200_w4a16_experts_params_t* params,

@@ -56,8 +56,10 @@ struct alignas(128) ExWorkspace {
   uint8_t map_a[128];    // 16-bit [rows, K], 128-byte swizzle, box 64 x 64
   uint8_t map_w[128];    // u8 [experts * N, K/2], 64-byte swizzle, box 64 x 128
   uint8_t map_out[128];  // 16-bit [rows, N], no swizzle, box 128 x 64
-  uint32_t status[32];
+  uint32_t status[18];
+  uint32_t note[14];     // what prepare() built the maps for
 };
+constexpr uint32_t kExNoteMagic = 0x45585034u;
 
 __device__ __forceinline__ void ex_report(ExWorkspace* ws, uint32_t code, uint32_t info) {
   if (atomicCAS(&ws->status[0], 0u, code) == 0u) ws->status[1] = info;
@@ -146,8 +148,8 @@ __device__ __forceinline__ void unpack8_minus(uint32_t v, uint32_t offset, uint3
 
 template <int AROWS, bool BF16, bool ZEROS>
 __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t* __restrict__ zeros,
-                             const int32_t* __restrict__ offsets, uint16_t* __restrict__ out, ExWorkspace* __restrict__ ws,
-                             int rows, int N, int K, int group, int ldo, int experts) {
+                             const int32_t* __restrict__ offsets, uint16_t* __restrict__ out, const void* a, const void* wq,
+                             ExWorkspace* __restrict__ ws, int rows, int N, int K, int group, int lda, int ldo, int experts) {
   using X = Ex<AROWS>;
   constexpr int kGroups = X::kGroups;
   extern __shared__ uint8_t smem_raw[];
@@ -197,6 +199,17 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
   }
   grid_dependency_wait();
   if (warp == 1) {  // the tile list: rows and tiles before each expert
+    // A workspace that was not prepared for these operands holds no maps, or others': nothing is copied through it.
+    const auto low = [](const void* p) { return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)); };
+    const auto high = [](const void* p) { return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) >> 32); };
+    const uint32_t want[14] = {kExNoteMagic, BF16, static_cast<uint32_t>(rows), static_cast<uint32_t>(N), static_cast<uint32_t>(K),
+                               static_cast<uint32_t>(lda), static_cast<uint32_t>(ldo), static_cast<uint32_t>(experts),
+                               low(a), high(a), low(wq), high(wq), low(out), high(out)};
+    bool same = true;
+#pragma unroll
+    for (int i = 0; i < 14; ++i) same = same && (lane != i || ws->note[i] == want[i]);
+    const bool prepared = __all_sync(0xffffffffu, same);
+    if (!prepared && lane == 0 && blockIdx.x == 0) ex_report(ws, kStatusBadArgument, 0);
     int sum = 0;
     for (int e0 = 0; e0 < experts; e0 += 32) {
       const int e = e0 + lane;
@@ -219,7 +232,7 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
       sum += __shfl_sync(0xffffffffu, incl, 31);
     }
     if (lane == 0) {
-      tile_first[experts] = sum;
+      tile_first[experts] = prepared ? sum : 0;
       row_first[experts] = min(max(offsets[experts], 0), rows);
     }
   }
@@ -598,14 +611,17 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
 
 }  // namespace b200
 
-// Bindings: scales, zero points (NULL: signed weights), row offsets, result, workspace.
+// Bindings: scales, zero points (NULL: signed weights), row offsets, result, activations, weights (both reached through the
+// workspace's maps; named to be compared with its note), workspace.
 #define B200_W4A16_EXPERTS(NAME, AROWS, BF16)                                                                              \
   extern "C" __global__ void __launch_bounds__(b200::Ex<AROWS>::kThreads, 1)                                               \
-      NAME(const uint16_t* scales, const uint16_t* zeros, const int32_t* offsets, uint16_t* out, void* ws, int rows, int N,  \
-           int K, int group, int ldo, int experts) {                                                                       \
+      NAME(const uint16_t* scales, const uint16_t* zeros, const int32_t* offsets, uint16_t* out, const void* a,            \
+           const void* wq, void* ws, int rows, int N, int K, int group, int lda, int ldo, int experts) {                   \
     b200::ExWorkspace* w = reinterpret_cast<b200::ExWorkspace*>(ws);                                                       \
-    if (zeros) b200::experts_body<AROWS, BF16, true>(scales, zeros, offsets, out, w, rows, N, K, group, ldo, experts);     \
-    else b200::experts_body<AROWS, BF16, false>(scales, zeros, offsets, out, w, rows, N, K, group, ldo, experts);          \
+    if (zeros)                                                                                                             \
+      b200::experts_body<AROWS, BF16, true>(scales, zeros, offsets, out, a, wq, w, rows, N, K, group, lda, ldo, experts);  \
+    else                                                                                                                   \
+      b200::experts_body<AROWS, BF16, false>(scales, zeros, offsets, out, a, wq, w, rows, N, K, group, lda, ldo, experts); \
   }
 B200_W4A16_EXPERTS(b200_w4a16_experts_f16, 256, false)
 B200_W4A16_EXPERTS(b200_w4a16_experts_bf16, 256, true)

@@ -131,15 +131,6 @@ def _vp(x) -> C.c_void_p:
     raise TypeError(type(x))
 
 
-def _address(x) -> int:
-    """Device address of a torch tensor, a DeviceBuffer, an int, or None."""
-    if x is None:
-        return 0
-    if hasattr(x, "data_ptr"):
-        return x.data_ptr()
-    return _vp(x).value or 0
-
-
 class DeviceBuffer:
     """A raw device allocation (what a HAL buffer resolves to before a launch)."""
 
@@ -219,6 +210,7 @@ class Context:
         h = C.c_void_p()
         check(lib.iree_b200_context_create(C.c_int32(device_ordinal), cubin.encode(), C.byref(h)))
         self.handle = h
+        self.ordinal = device_ordinal
         self.device = C.c_void_p(lib.iree_b200_context_device(h))
         self.executable = C.c_void_p(lib.iree_b200_context_executable(h))
         self.command_buffer = C.c_void_p(lib.iree_b200_context_command_buffer(h))
@@ -375,11 +367,33 @@ class Context:
         check(library().iree_b200_w4a16_wait_arrivals(self.handle, _vp(own_flags), _vp(ws), C.c_int32(world),
                                                       C.c_int32(epoch)))
 
+    def _on_device(self, x, element_bytes: int) -> int:
+        """Address of an array of the expert layer's calls: a torch tensor on this device with elements of that size, a
+        DeviceBuffer of this context, a device address, or None."""
+        if x is None:
+            return 0
+        if hasattr(x, "data_ptr"):
+            if x.get_device() != self.ordinal or x.element_size() != element_bytes:
+                raise IreeB200Error(3, "expected %d-byte elements on device %d, got %s on %s" % (element_bytes, self.ordinal,
+                                                                                             x.dtype, x.device))
+            return x.data_ptr()
+        if isinstance(x, DeviceBuffer):
+            if x.ctx.ordinal != self.ordinal:
+                raise IreeB200Error(3, "the buffer is on device %d, not %d" % (x.ctx.ordinal, self.ordinal))
+            return x.ptr
+        if isinstance(x, int):
+            return x
+        raise IreeB200Error(3, "expected a device array, got %s" % type(x).__name__)
+
+    def _scratch(self, x) -> int:
+        return self._on_device(x, x.element_size()) if hasattr(x, "element_size") else self._on_device(x, 1)
+
     # 4-bit matrix-vector products and the expert layer. Arrays: torch tensors on this device, DeviceBuffers or addresses.
     def w4a16_matvec(self, params: W4A16MatvecParams, a, wq, scales, zeros, out) -> None:
         """out[M, N] = a[M, K] x w[N, K]^T for up to 16 rows; ``zeros`` None: signed weights."""
-        check(library().iree_b200_w4a16_matvec(self.handle, C.addressof(params), _address(a), _address(wq), _address(scales),
-                                               _address(zeros), _address(out)))
+        check(library().iree_b200_w4a16_matvec(
+            self.handle, C.addressof(params), self._on_device(a, 2), self._on_device(wq, 1),
+            self._on_device(scales, 2), self._on_device(zeros, 2), self._on_device(out, 2)))
 
     def w4a16_experts_workspace(self, params: W4A16ExpertsParams) -> DeviceBuffer:
         nbytes = int(library().iree_b200_w4a16_experts_workspace_bytes(C.byref(params)))
@@ -387,19 +401,22 @@ class Context:
 
     def w4a16_experts_prepare(self, params: W4A16ExpertsParams, a, wq, out, ws) -> int:
         variant = C.c_int32()
-        check(library().iree_b200_w4a16_experts_prepare(self.handle, C.byref(params), _vp(a), _vp(wq), _vp(out), _vp(ws),
-                                                        C.byref(variant)))
+        check(library().iree_b200_w4a16_experts_prepare(
+            self.handle, C.byref(params), C.c_void_p(self._on_device(a, 2)), C.c_void_p(self._on_device(wq, 1)),
+            C.c_void_p(self._on_device(out, 2)), C.c_void_p(self._scratch(ws)), C.byref(variant)))
         return variant.value
 
     def w4a16_experts_run(self, params: W4A16ExpertsParams, a, wq, scales, zeros, offsets, out, ws, variant: int) -> None:
         check(library().iree_b200_w4a16_experts_run(
-            self.handle, C.addressof(params), _address(a), _address(wq), _address(scales), _address(zeros), _address(offsets),
-            _address(out), _address(ws), variant))
+            self.handle, C.addressof(params), self._on_device(a, 2), self._on_device(wq, 1),
+            self._on_device(scales, 2), self._on_device(zeros, 2), self._on_device(offsets, 4),
+            self._on_device(out, 2), self._scratch(ws), variant))
 
     def w4a16_experts(self, params: W4A16ExpertsParams, a, wq, scales, zeros, offsets, out, ws) -> None:
         check(library().iree_b200_w4a16_experts(
-            self.handle, C.addressof(params), _address(a), _address(wq), _address(scales), _address(zeros), _address(offsets),
-            _address(out), _address(ws)))
+            self.handle, C.addressof(params), self._on_device(a, 2), self._on_device(wq, 1),
+            self._on_device(scales, 2), self._on_device(zeros, 2), self._on_device(offsets, 4),
+            self._on_device(out, 2), self._scratch(ws)))
 
     def expert_dispatch_workspace(self, params: ExpertRowsParams) -> Optional[DeviceBuffer]:
         """None where the dispatch needs none."""
@@ -408,23 +425,27 @@ class Context:
 
     def expert_dispatch(self, params: ExpertRowsParams, expert_ids, x, offsets, position, order, rows, ws) -> None:
         """Sorts (token, slot) pairs by expert and copies the tokens' rows there."""
-        check(library().iree_b200_expert_dispatch(self.handle, C.addressof(params), _address(expert_ids), _address(x),
-                                                  _address(offsets), _address(position), _address(order), _address(rows),
-                                                  _address(ws)))
+        check(library().iree_b200_expert_dispatch(
+            self.handle, C.addressof(params), self._on_device(expert_ids, 4), self._on_device(x, 2),
+            self._on_device(offsets, 4), self._on_device(position, 4), self._on_device(order, 4),
+            self._on_device(rows, 2), self._scratch(ws)))
 
     def expert_dispatch_backward(self, params: ExpertRowsParams, drows, position, dx) -> None:
-        check(library().iree_b200_expert_dispatch_backward(self.handle, C.addressof(params), _address(drows),
-                                                           _address(position), _address(dx)))
+        check(library().iree_b200_expert_dispatch_backward(
+            self.handle, C.addressof(params), self._on_device(drows, 2), self._on_device(position, 4),
+            self._on_device(dx, 2)))
 
     def expert_combine(self, params: ExpertRowsParams, rows, weights, position, out) -> None:
         """out[t] = sum of weights[t, j] * rows[position[t, j]]."""
-        check(library().iree_b200_expert_combine(self.handle, C.addressof(params), _address(rows), _address(weights),
-                                                 _address(position), _address(out)))
+        check(library().iree_b200_expert_combine(
+            self.handle, C.addressof(params), self._on_device(rows, 2), self._on_device(weights, 4),
+            self._on_device(position, 4), self._on_device(out, 2)))
 
     def expert_combine_backward(self, params: ExpertRowsParams, dout, rows, weights, position, drows, dweights) -> None:
         check(library().iree_b200_expert_combine_backward(
-            self.handle, C.addressof(params), _address(dout), _address(rows), _address(weights), _address(position),
-            _address(drows), _address(dweights)))
+            self.handle, C.addressof(params), self._on_device(dout, 2), self._on_device(rows, 2),
+            self._on_device(weights, 4), self._on_device(position, 4), self._on_device(drows, 2),
+            self._on_device(dweights, 4)))
 
     def w4a16_host(self, params: W4A16Params, a, wq, scales, out) -> None:
         check(library().iree_b200_w4a16_host(self.handle, C.byref(params), _vp(a), _vp(wq), _vp(scales), _vp(out)))

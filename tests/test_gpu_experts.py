@@ -391,7 +391,7 @@ def check_experts(ctx, kind, counts, N, K, group, zeros, spare=0, variant=0, see
 
 EXPERT_SHAPES = [  # rows per expert, N, K, group
     ([1], 40, 64, 32), ([0, 3, 0, 1, 9], 75, 160, 32), ([2, 0, 0, 30], 130, 256, 64), ([0] * 70 + [5] + [0] * 9, 33, 128, 128),
-    ([17, 1, 8, 16], 96, 480, 96), ([1] * 300, 20, 64, 64), ([100, 2], 200, 1024, 128), ([3, 4, 5, 6], 1003, 4128, 32),
+    ([5, 14], 7, 32, 32), ([17, 1, 8, 16], 96, 480, 96), ([1] * 300, 20, 64, 64), ([100, 2], 200, 1024, 128), ([3, 4, 5, 6], 1003, 4128, 32),
 ]
 
 
@@ -429,6 +429,40 @@ def test_experts_tensor_refuses_what_its_copies_cannot_reach(ctx):
     for layout in (dict(pad_a=1), dict(pad_out=1), dict(offset=4)):
         with pytest.raises(ib.IreeB200Error, match="INVALID_ARGUMENT"):
             run_experts(ctx, F16, [4, 4], 8, w, 32, a, variant=ib.W4A16_EXPERTS_TENSOR, **layout)
+
+
+def test_experts_tensor_refuses_a_workspace_of_other_operands(ctx):
+    """run() on a workspace that was never prepared, or for another result: nothing is computed and the status says so."""
+    rng = np.random.default_rng(4)
+    E, rows, N, K = 2, 40, 64, 128
+    w = Weights(rng, F16, E, N, K, 128, False)
+    da, dw, ds, doff = (upload(ctx, v) for v in (to_bits(rng.standard_normal((rows, K)), F16), w.wq, w.scales, offsets_of([18, 22])))
+    do, other = (ctx.alloc(2 * rows * N).fill(0x5A) for _ in range(2))
+    p = ib.W4A16ExpertsParams(F16, E, rows, N, K, 128, K, N, ib.W4A16_EXPERTS_TENSOR)
+    fresh, ready = ctx.w4a16_experts_workspace(p), ctx.w4a16_experts_workspace(p)
+    assert ctx.w4a16_experts_prepare(p, da, dw, do, ready) == ib.W4A16_EXPERTS_TENSOR
+    for ws, out in ((fresh, do), (ready, other)):
+        ctx.w4a16_experts_run(p, da, dw, ds, None, doff, out, ws, ib.W4A16_EXPERTS_TENSOR)
+        with pytest.raises(ib.IreeB200Error, match="INVALID_ARGUMENT"):
+            ctx.workspace_status(ws)
+        assert (out.download(np.uint8, (2 * rows * N,)) == 0x5A).all()
+    free(da, dw, ds, doff, do, other, fresh, ready)
+
+
+def test_arrays_of_another_kind_are_refused(ctx):
+    """Host arrays, elements of another size and tensors elsewhere would be read as something they are not."""
+    import torch
+    p = ib.ExpertRowsParams(F16, 2, 2, 4, 0, 8, 8, 8)
+    t = dict(ids=torch.zeros(2, 2, dtype=torch.int32), x=torch.zeros(2, 8, dtype=torch.float16), offsets=torch.zeros(5, dtype=torch.int32),
+             position=torch.zeros(2, 2, dtype=torch.int32), order=torch.zeros(4, dtype=torch.int32), rows=torch.zeros(4, 8, dtype=torch.float16))
+    good = [v.cuda() for v in t.values()]
+    torch.cuda.synchronize()
+    ctx.expert_dispatch(p, *good, None)
+    ctx.synchronize()
+    for i, v in enumerate(t.values()):
+        for bad in (v, v.numpy(), good[i].to(torch.float64 if v.is_floating_point() else torch.int64)):
+            with pytest.raises(ib.IreeB200Error, match="INVALID_ARGUMENT"):
+                ctx.expert_dispatch(p, *good[:i], bad, *good[i + 1:], None)
 
 
 def layer_buffers(ctx, rng, T, k, E, D, H, group, kind):
