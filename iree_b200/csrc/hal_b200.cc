@@ -1770,7 +1770,7 @@ constexpr uint32_t kStreamSmemBytes = 16 * (2 * 2048 + 2 * 1024) + 2 * (54 * 102
 constexpr uint32_t kExpertsR64SmemBytes = 1024 + 8 * 8192 + 12 * 8192 + 2 * 16384 + 512 + 2 * 1025 * 4 + 56;
 constexpr uint32_t kExpertsSmemBytes = 1024 + 4 * 32768 + 6 * 8192 + 2 * 16384 + 512 + 2 * 1025 * 4 + 56;
 // b200_expert_route: per expert a next row, its start, an offset and 16 warps' counts, and the rows of 512 slots
-constexpr uint32_t kRouteSmemBytes = 4 * (3 * 1024 + 1 + 512) + 2 * 16 * 1024;
+constexpr uint32_t kRouteSmemBytes = (4 + 4 + 4 + 2 * 16) * 1024 + 4 * (1 + 512);
 constexpr int kMaxExperts = 1024;
 constexpr uint32_t kExpertsNoteMagic = 0x45585034u;
 constexpr int kMaxSlots = 256;
@@ -2732,10 +2732,10 @@ static iree_b200_status_t rows_check(const void* a, const void* b, const void* c
   return IREE_B200_STATUS_OK;
 }
 
-// Runs of tokens (grid x) and column parts (grid y) of the routing kernel: two CTAs per SM over the runs, and
+// Runs of tokens (grid x) and column parts (grid y) of the routing kernel: one CTA per SM over the runs, and
 // where there are few tokens their rows cut into parts.
 static void route_grid(const iree_b200_expert_rows_params_t* p, int sms, int* run, int* runs, int* part_width, int* parts) {
-  const int want = 2 * sms;
+  const int want = sms;
   *run = p->tokens > want ? (p->tokens + want - 1) / want : 1;
   *runs = p->tokens ? (p->tokens + *run - 1) / *run : 1;
   int cut = sms / *runs;
@@ -2750,8 +2750,8 @@ static void route_grid(const iree_b200_expert_rows_params_t* p, int sms, int* ru
 size_t iree_b200_expert_dispatch_workspace_bytes(const iree_b200_expert_rows_params_t* params) {
   if (rows_validate(params) != IREE_B200_STATUS_OK) return 0;
   if (static_cast<int64_t>(params->tokens) * params->slots <= kRouteSingleSlots) return 0;
-  // one histogram per run and their sum; at most 2 x 148 runs on any device this library drives, whatever SMs are reserved
-  return static_cast<size_t>(2 * 148 + 1) * params->experts * sizeof(int32_t);
+  // one histogram per run and their sum; at most 148 runs, whatever SMs are reserved
+  return static_cast<size_t>(148 + 1) * params->experts * sizeof(int32_t);
 }
 
 iree_b200_status_t iree_b200_expert_dispatch(iree_b200_context_t* context, const iree_b200_expert_rows_params_t* params,
