@@ -110,6 +110,7 @@ def check_matvec(ctx, kind, M, N, K, group, zeros, seed=0, integer_zeros=True, *
 @pytest.mark.parametrize("M, N, K, group", [
     (1, 1, 32, 32), (1, 17, 64, 64), (2, 75, 160, 32), (3, 1003, 1376, 32), (7, 250, 480, 96), (8, 333, 512, 128),
     (9, 160, 192, 64), (16, 300, 1024, 256), (5, 40, 8320, 128), (16, 70, 4224, 64), (11, 19, 8224, 32), (1, 2400, 4096, 128),
+    (2, 5, 65536, 64), (12, 33, 40960, 128),
 ])
 def test_matvec(ctx, kind, zeros, M, N, K, group):
     check_matvec(ctx, kind, M, N, K, group, zeros)
@@ -429,6 +430,62 @@ def test_experts_tensor_refuses_what_its_copies_cannot_reach(ctx):
     for layout in (dict(pad_a=1), dict(pad_out=1), dict(offset=4)):
         with pytest.raises(ib.IreeB200Error, match="INVALID_ARGUMENT"):
             run_experts(ctx, F16, [4, 4], 8, w, 32, a, variant=ib.W4A16_EXPERTS_TENSOR, **layout)
+
+
+@pytest.mark.parametrize("variant", [ib.W4A16_EXPERTS_STREAM, ib.W4A16_EXPERTS_TENSOR])
+def test_experts_whose_weights_pass_four_gigabytes(ctx, variant):
+    """The last expert's weights and scales start 7.4 GB and 0.23 GB into their arrays."""
+    import torch
+    rng = np.random.default_rng(8)
+    E, N, K, group, kind = 64, 28672, 8192, 128, F16
+    counts = [2] + [0] * (E - 2) + [21]
+    rows = sum(counts)
+    wq = torch.full((E, N, K // 2), 0x77, dtype=torch.uint8, device="cuda")
+    scales = torch.full((E, N, K // group), 0.0625, dtype=torch.float16, device="cuda")
+    last = torch.from_numpy(rng.integers(0, 256, (N, K // 2), dtype=np.uint8))
+    wq[-1].copy_(last)
+    scales[-1] = 0.03125
+    a = torch.from_numpy(rng.integers(-2, 3, (rows, K)).astype(np.float16)).cuda()
+    out = torch.zeros(rows, N, dtype=torch.float16, device="cuda")
+    offsets = torch.from_numpy(offsets_of(counts)).cuda()
+    torch.cuda.synchronize()
+    p = ib.W4A16ExpertsParams(kind, E, rows, N, K, group, K, N, variant)
+    ws = ctx.w4a16_experts_workspace(p)
+    ctx.w4a16_experts(p, a, wq, scales, None, offsets, out, ws)
+    ctx.synchronize()
+    ctx.workspace_status(ws)
+    # whole numbers times powers of two: every step before the last rounding is exact
+    pick = rng.integers(0, N, 200)
+    q = np.stack([last.numpy()[pick] & 15, last.numpy()[pick] >> 4], axis=-1).reshape(len(pick), K).astype(np.float64)
+    q[q >= 8] -= 16
+    a64, got = a.cpu().numpy().astype(np.float64), out.cpu().numpy()
+    assert (got[2:][:, pick] == (a64[2:] @ q.T * 0.03125).astype(np.float16)).all()
+    assert (got[:2] == (a64[:2].sum(1, keepdims=True) * 7 * 0.0625).astype(np.float16)).all()
+    ws.free()
+
+
+def test_rows_that_pass_four_gigabytes(ctx):
+    """2^20 rows of 2200: the last ones start 4.6 GB into their array."""
+    import torch
+    T, k, E, D = 1 << 19, 2, 16, 2200
+    g = torch.Generator(device="cuda").manual_seed(3)
+    x = torch.randint(-9, 10, (T, D), generator=g, device="cuda", dtype=torch.int16).to(torch.float16)
+    ids = torch.randint(0, E, (T, k), generator=g, device="cuda", dtype=torch.int32)
+    i32 = dict(dtype=torch.int32, device="cuda")
+    offsets, position, order = torch.zeros(E + 1, **i32), torch.zeros(T, k, **i32), torch.zeros(T * k, **i32)
+    rows, out = torch.zeros(T * k, D, dtype=torch.float16, device="cuda"), torch.zeros(T, D, dtype=torch.float16, device="cuda")
+    torch.cuda.synchronize()
+    p = ib.ExpertRowsParams(F16, T, k, E, 0, D, D, D)
+    ws = ctx.expert_dispatch_workspace(p)
+    ctx.expert_dispatch(p, ids, x, offsets, position, order, rows, ws)
+    ctx.expert_dispatch_backward(p, rows, position, out)
+    ctx.synchronize()
+    want = torch.sort(ids.reshape(-1).long(), stable=True).indices
+    assert (order.long() == want).all() and (position.reshape(-1)[want] == torch.arange(T * k, device="cuda")).all()
+    for lo in range(0, T * k, 1 << 17):       # in parts: the comparison's own memory
+        assert (rows[lo:lo + (1 << 17)] == x[want[lo:lo + (1 << 17)] // k]).all()
+    assert (out == x + x).all()
+    ws.free()
 
 
 def test_experts_tensor_refuses_a_workspace_of_other_operands(ctx):
