@@ -5,11 +5,11 @@
 //
 // The one rounding that is not the result's: a weight enters the tensor core as f16 or bf16, off by half a step of its own value
 // (with a fractional zero point q - z is rounded as well). Its error is random from weight to weight: together with the result's
-// rounding it measures sqrt(2) times the result's alone. Scaling group sums in f32 instead would need the accumulator back in
+// rounding it measures 1.3 times the result's alone (root mean square, relative: bf16 0.0022 for 0.0017, f16 0.00028 for 0.00021). Scaling group sums in f32 instead would need the accumulator back in
 // registers for every group, four times the tensor time. Sums are f32 in tensor memory.
 //
 // Roles as in b200_w4a16_gemm_wt: warp 0 fetches activation tiles (TMA, 128-byte swizzle, boxes of 64 rows x 64 K), warp 3 raw
-// weight tiles (128 rows x 128 K), warps 8-15 expand weights into tensor memory (a thread owns a weight row = a lane), one
+// weight tiles (128 rows x 128 K), warps 8 and up expand weights into tensor memory (a thread owns a weight row = a lane), one
 // thread of warp 1 issues the matrix instructions two K blocks at a time, warps 4-7 bring the transposed accumulator back.
 // What differs: tiles are (expert, 128 weight rows, up to 256 activation rows), listed from the device's row offsets by every
 // CTA itself. An expert's rows are cut into equal parts of a multiple of 16 (260 rows are 2 x 144, not 256 + 16), and the
