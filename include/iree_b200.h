@@ -628,7 +628,7 @@ iree_b200_status_t iree_b200_expert_dispatch_backward(iree_b200_context_t* conte
 iree_b200_status_t iree_b200_expert_combine(iree_b200_context_t* context, const iree_b200_expert_rows_params_t* params,
                                             const void* rows, const float* weights, const int32_t* position, void* out);
 /* Its gradients: drows[position[t, j]] = weights[t, j] * dout[t] (rows behind the last one are left as they were),
- * dweights[t, j] = <dout[t], rows[position[t, j]]> (0 for a dropped slot). drows may not overlap rows. */
+ * dweights[t, j] = <dout[t], rows[position[t, j]]> (0 for a dropped slot). drows may overlap neither rows nor dout. */
 iree_b200_status_t iree_b200_expert_combine_backward(iree_b200_context_t* context,
                                                      const iree_b200_expert_rows_params_t* params, const void* dout,
                                                      const void* rows, const float* weights, const int32_t* position,

@@ -367,15 +367,22 @@ class Context:
         check(library().iree_b200_w4a16_wait_arrivals(self.handle, _vp(own_flags), _vp(ws), C.c_int32(world),
                                                       C.c_int32(epoch)))
 
-    def _on_device(self, x, element_bytes: int) -> int:
+    def _on_device(self, x, element_bytes: int, pitched: bool = False) -> int:
         """Address of an array of the expert layer's calls: a torch tensor on this device with elements of that size, a
-        DeviceBuffer of this context, a device address, or None."""
+        DeviceBuffer of this context, a device address, or None. Rows whose pitch the parameters give (``pitched``) need
+        adjacent elements, other tensors have no gaps at all."""
         if x is None:
             return 0
-        if hasattr(x, "data_ptr"):
-            if x.get_device() != self.ordinal or x.element_size() != element_bytes:
+        try:
+            device = x.get_device()
+        except AttributeError:
+            device = None
+        if device is not None:
+            if device != self.ordinal or x.itemsize != element_bytes:
                 raise IreeB200Error(3, "expected %d-byte elements on device %d, got %s on %s" % (element_bytes, self.ordinal,
                                                                                              x.dtype, x.device))
+            if not x.is_contiguous() and not (pitched and x.dim() == 2 and x.stride(1) == 1):
+                raise IreeB200Error(3, "strides %s of a %s: its elements are not adjacent" % (x.stride(), tuple(x.shape)))
             return x.data_ptr()
         if isinstance(x, DeviceBuffer):
             if x.ctx.ordinal != self.ordinal:
@@ -392,8 +399,8 @@ class Context:
     def w4a16_matvec(self, params: W4A16MatvecParams, a, wq, scales, zeros, out) -> None:
         """out[M, N] = a[M, K] x w[N, K]^T for up to 16 rows; ``zeros`` None: signed weights."""
         check(library().iree_b200_w4a16_matvec(
-            self.handle, C.addressof(params), self._on_device(a, 2), self._on_device(wq, 1),
-            self._on_device(scales, 2), self._on_device(zeros, 2), self._on_device(out, 2)))
+            self.handle, C.addressof(params), self._on_device(a, 2, True), self._on_device(wq, 1),
+            self._on_device(scales, 2), self._on_device(zeros, 2), self._on_device(out, 2, True)))
 
     def w4a16_experts_workspace(self, params: W4A16ExpertsParams) -> DeviceBuffer:
         nbytes = int(library().iree_b200_w4a16_experts_workspace_bytes(C.byref(params)))
@@ -402,21 +409,21 @@ class Context:
     def w4a16_experts_prepare(self, params: W4A16ExpertsParams, a, wq, out, ws) -> int:
         variant = C.c_int32()
         check(library().iree_b200_w4a16_experts_prepare(
-            self.handle, C.byref(params), C.c_void_p(self._on_device(a, 2)), C.c_void_p(self._on_device(wq, 1)),
-            C.c_void_p(self._on_device(out, 2)), C.c_void_p(self._scratch(ws)), C.byref(variant)))
+            self.handle, C.byref(params), C.c_void_p(self._on_device(a, 2, True)), C.c_void_p(self._on_device(wq, 1)),
+            C.c_void_p(self._on_device(out, 2, True)), C.c_void_p(self._scratch(ws)), C.byref(variant)))
         return variant.value
 
     def w4a16_experts_run(self, params: W4A16ExpertsParams, a, wq, scales, zeros, offsets, out, ws, variant: int) -> None:
         check(library().iree_b200_w4a16_experts_run(
-            self.handle, C.addressof(params), self._on_device(a, 2), self._on_device(wq, 1),
+            self.handle, C.addressof(params), self._on_device(a, 2, True), self._on_device(wq, 1),
             self._on_device(scales, 2), self._on_device(zeros, 2), self._on_device(offsets, 4),
-            self._on_device(out, 2), self._scratch(ws), variant))
+            self._on_device(out, 2, True), self._scratch(ws), variant))
 
     def w4a16_experts(self, params: W4A16ExpertsParams, a, wq, scales, zeros, offsets, out, ws) -> None:
         check(library().iree_b200_w4a16_experts(
-            self.handle, C.addressof(params), self._on_device(a, 2), self._on_device(wq, 1),
+            self.handle, C.addressof(params), self._on_device(a, 2, True), self._on_device(wq, 1),
             self._on_device(scales, 2), self._on_device(zeros, 2), self._on_device(offsets, 4),
-            self._on_device(out, 2), self._scratch(ws)))
+            self._on_device(out, 2, True), self._scratch(ws)))
 
     def expert_dispatch_workspace(self, params: ExpertRowsParams) -> Optional[DeviceBuffer]:
         """None where the dispatch needs none."""
@@ -426,25 +433,25 @@ class Context:
     def expert_dispatch(self, params: ExpertRowsParams, expert_ids, x, offsets, position, order, rows, ws) -> None:
         """Sorts (token, slot) pairs by expert and copies the tokens' rows there."""
         check(library().iree_b200_expert_dispatch(
-            self.handle, C.addressof(params), self._on_device(expert_ids, 4), self._on_device(x, 2),
+            self.handle, C.addressof(params), self._on_device(expert_ids, 4), self._on_device(x, 2, True),
             self._on_device(offsets, 4), self._on_device(position, 4), self._on_device(order, 4),
-            self._on_device(rows, 2), self._scratch(ws)))
+            self._on_device(rows, 2, True), self._scratch(ws)))
 
     def expert_dispatch_backward(self, params: ExpertRowsParams, drows, position, dx) -> None:
         check(library().iree_b200_expert_dispatch_backward(
-            self.handle, C.addressof(params), self._on_device(drows, 2), self._on_device(position, 4),
-            self._on_device(dx, 2)))
+            self.handle, C.addressof(params), self._on_device(drows, 2, True), self._on_device(position, 4),
+            self._on_device(dx, 2, True)))
 
     def expert_combine(self, params: ExpertRowsParams, rows, weights, position, out) -> None:
         """out[t] = sum of weights[t, j] * rows[position[t, j]]."""
         check(library().iree_b200_expert_combine(
-            self.handle, C.addressof(params), self._on_device(rows, 2), self._on_device(weights, 4),
-            self._on_device(position, 4), self._on_device(out, 2)))
+            self.handle, C.addressof(params), self._on_device(rows, 2, True), self._on_device(weights, 4),
+            self._on_device(position, 4), self._on_device(out, 2, True)))
 
     def expert_combine_backward(self, params: ExpertRowsParams, dout, rows, weights, position, drows, dweights) -> None:
         check(library().iree_b200_expert_combine_backward(
-            self.handle, C.addressof(params), self._on_device(dout, 2), self._on_device(rows, 2),
-            self._on_device(weights, 4), self._on_device(position, 4), self._on_device(drows, 2),
+            self.handle, C.addressof(params), self._on_device(dout, 2, True), self._on_device(rows, 2, True),
+            self._on_device(weights, 4), self._on_device(position, 4), self._on_device(drows, 2, True),
             self._on_device(dweights, 4)))
 
     def w4a16_host(self, params: W4A16Params, a, wq, scales, out) -> None:

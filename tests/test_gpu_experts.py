@@ -522,6 +522,38 @@ def test_arrays_of_another_kind_are_refused(ctx):
                 ctx.expert_dispatch(p, *good[:i], bad, *good[i + 1:], None)
 
 
+def test_arrays_with_gaps_are_refused(ctx):
+    """Tables, weights and scales have no pitch; rows have one, but adjacent elements."""
+    import torch
+    T, k, E, D = 3, 2, 4, 16
+    p = ib.ExpertRowsParams(F16, T, k, E, 0, D, 2 * D, 3 * D)
+    i32, half = dict(dtype=torch.int32, device="cuda"), dict(dtype=torch.float16, device="cuda")
+    ids = torch.tensor([[1, 0], [3, 9], [2, 2]], **i32)
+    x = torch.arange(T * 2 * D, **half).reshape(T, 2 * D)[:, :D]
+    offsets, position, order = torch.zeros(E + 1, **i32), torch.zeros(T, k, **i32), torch.zeros(T * k, **i32)
+    rows = torch.zeros(T * k, 3 * D, **half)[:, :D]
+    torch.cuda.synchronize()
+    good = [ids, x, offsets, position, order, rows]
+    ctx.expert_dispatch(p, *good, None)
+    ctx.synchronize()
+    assert position.tolist() == [[1, 0], [4, -1], [2, 3]]
+    assert (rows[:5] == x[torch.tensor([0, 0, 2, 2, 1], device="cuda")]).all()
+    for i, v in enumerate(good):
+        # the same shape, but every other element; for rows also with whole planes between them
+        gaps = torch.zeros(*v.shape, 2, dtype=v.dtype, device="cuda")[..., 0]
+        planes = torch.zeros(2, *v.shape, dtype=v.dtype, device="cuda")[:, :1]
+        for bad in (gaps, planes):
+            with pytest.raises(ib.IreeB200Error, match="INVALID_ARGUMENT"):
+                ctx.expert_dispatch(p, *good[:i], bad, *good[i + 1:], None)
+    weights = torch.ones(T, 2 * k, device="cuda")[:, :k]
+    out = torch.zeros(T, 2 * D, **half)[:, :D]
+    with pytest.raises(ib.IreeB200Error, match="INVALID_ARGUMENT"):
+        ctx.expert_combine(p, rows, weights, position, out)
+    ctx.expert_combine(p, rows, weights.contiguous(), position, out)
+    ctx.synchronize()
+    assert (out == x * torch.tensor([[2], [1], [2]], **half)).all()
+
+
 def layer_buffers(ctx, rng, T, k, E, D, H, group, kind):
     x = to_bits(rng.standard_normal((T, D)), kind)
     ids = np.stack([rng.permutation(E)[:k] for _ in range(T)]).astype(np.int32)
