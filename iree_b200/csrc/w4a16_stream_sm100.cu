@@ -27,6 +27,7 @@
 
 #include "sm100_ptx.cuh"
 #include "w4a16_decode.cuh"
+#include "w4a16_stream_list.h"
 
 namespace b200 {
 
@@ -279,8 +280,7 @@ __device__ void stream_body(const StreamArgs& p) {
     passes = pass_first[p.experts];
   }
   const int64_t total = passes * p.N;  // weight rows to be read, over all passes
-  const int64_t share = total >> 32 ? (total + gridDim.x - 1) / gridDim.x
-                                    : (static_cast<uint32_t>(total) + gridDim.x - 1) / gridDim.x;
+  const int64_t share = list_share(total, gridDim.x);
   StreamWalk& walk = *reinterpret_cast<StreamWalk*>(smem_raw + kStreamWalkOffset + warp * kStreamWalkBytes);
   if (lane == 0) {
     StreamList list = {p.offsets ? pass_first : nullptr, row_first, 0, 0, 0, p.N, p.M, p.experts, kCols, 0, 0};
