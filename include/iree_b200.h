@@ -577,7 +577,9 @@ int32_t iree_b200_w4a16_host_plan(const iree_b200_w4a16_params_t* params, int32_
  * wq is [N, K/2] bytes (element 2i in the low nibble of byte i, as for iree_b200_w4a16), scales and zeros are [N, K/group]
  * in the kind's type. Sums are f32 and the result is rounded once. A row of activations that
  * is not finite gives results that are not (the streaming kernels: NaN where the exact sum is an infinity), and only that row:
- * no result depends on other rows or on the memory behind the last one. Every call queues work on the context's stream and returns; it may
+ * no result depends on other rows or on the memory behind the last one. Every finite activation is good for every finite result
+ * (zero points up to 128 in magnitude); the streaming kernels hold bf16 sums at 2^-15 of their value, so that results below 2^-111
+ * carry an absolute error of up to (K / 32 + 16) 2^-135 beside their rounding. Every call queues work on the context's stream and returns; it may
  * be recorded into a graph (begin_graph); calls share no scratch but the workspace they are given. All pointers are device
  * pointers: wq on a 16-byte, scales / zeros / activations / results on a 2-byte, index and f32 arrays on a 4-byte boundary
  * (INVALID_ARGUMENT otherwise). Activations, rows and results on 16-byte boundaries with pitches of whole 16-byte pieces

@@ -9,8 +9,11 @@
 //   v = sum_k a q' - z' sum_k a,   total += s v      all in f32; q' is the stored nibble (top bit flipped when it is signed,
 //                                                    z' = 8 then), so only the result is rounded to 16 bits.
 // A nibble becomes a 16-bit float by a shift and one logic operation for two weights: under the exponent of 64 (f16: its bits
-// land in mantissa bits 4..7) or 128 (bf16: bits 0..3), and z' grows by that much; the part that cancels is at most 158 / 15 of
-// the sum it leaves, 2^-20 of it in f32. (f16 subnormals, q 2^-24 as stored, would spare the shifts; but the tensor core
+// land in mantissa bits 4..7) or 2^-8 (bf16: bits 0..3, so it reads 2^-15 (128 + q')), and z' grows by 64 or 128; the part that
+// cancels is at most 158 / 15 of the sum it leaves, 2^-20 of it in f32. In bf16 everything up to the result is kept 2^-15 times
+// its value, which costs nothing (sums of activations are formed that way, the result is multiplied once): activations reach
+// f32's largest numbers, and 128 of them times 143 would pass it where the scaled sum is a number again. What that takes from
+// the other end: sums below 2^-111 round in steps of 2^-149 of f32's subnormals, 2^-134 of the value. (f16 subnormals, q 2^-24 as stored, would spare the shifts; but the tensor core
 // aligns products by their exponent fields, and sums lost up to six more bits there.) The accumulator starts
 // at minus that offset times the sum of a.
 //
@@ -47,6 +50,7 @@ constexpr int kStreamWalkOffset = kStreamTableOffset + 2 * (kStreamMaxExperts + 
 constexpr int kStreamWalkBytes = 304;              // per warp
 constexpr int kStreamSmemBytes = kStreamWalkOffset + kStreamWarps * kStreamWalkBytes;
 static_assert(kStreamSmemBytes <= 232448, "per-CTA shared memory limit");
+constexpr float kStreamBf16Unit = 1.f / 32768.f;   // what bf16 sums are held in
 
 // a / b for 0 <= a < 2^16, 0 < b <= 2^10: (a + 1/2) / b is at least 1 / 2b from a whole number, far more than the error.
 __device__ __forceinline__ int small_div(int a, int b) {
@@ -302,8 +306,9 @@ __device__ void stream_body(const StreamArgs& p) {
   }
   if (!p.offsets && !p.weights_ahead) grid_dependency_wait();
   const uint32_t mask = BF16 ? 0x000f000fu : 0x00f000f0u;
-  const uint32_t under = BF16 ? (p.zeros ? 0x43004300u : 0x43084308u) : (p.zeros ? 0x54005400u : 0x54805480u);
-  // what the unpacked nibbles stand above their values: of all of them, or without the zero points
+  const uint32_t under = BF16 ? (p.zeros ? 0x3b803b80u : 0x3b883b88u) : (p.zeros ? 0x54005400u : 0x54805480u);
+  // what the unpacked nibbles stand above their values (bf16: in units of kStreamBf16Unit): of all of them, or without the zero
+  // points
   const float above = (BF16 ? 128.f : 64.f) + (p.zeros ? 0.f : 8.f);
 
     // ---- unit sequence of this warp: (batch, slice, its run of the slice's chunks), ahead of its use -----------------------
@@ -421,8 +426,11 @@ __device__ void stream_body(const StreamArgs& p) {
         const uint32_t words[4] = {v.x, v.y, v.z, v.w};
         float sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          sum += half_bits_to_float<BF16>(words[j] & 0xffffu) + half_bits_to_float<BF16>(words[j] >> 16);
+        for (int j = 0; j < 4; ++j) {
+          const float lo = half_bits_to_float<BF16>(words[j] & 0xffffu), hi = half_bits_to_float<BF16>(words[j] >> 16);
+          if (BF16) sum = fmaf(kStreamBf16Unit, lo, fmaf(kStreamBf16Unit, hi, sum));
+          else sum += lo + hi;
+        }
 #pragma unroll
         for (int d = 1; d < 4 * GQ; d <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
         if (c < padded) {
@@ -599,7 +607,7 @@ __device__ void stream_body(const StreamArgs& p) {
             float v = 0.f;
             for (int w = 0; w < b.wk; ++w) v += src[w * b.wn * 2 * kTile];
             uint16_t bits;
-            if (BF16) bits = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+            if (BF16) bits = __bfloat16_as_ushort(__float2bfloat16_rn(v * (1.f / kStreamBf16Unit)));
             else bits = __half_as_ushort(__float2half_rn(v));
             p.out[static_cast<int64_t>(b.a_row + m) * p.ldo + b.n0 + n] = bits;
           }

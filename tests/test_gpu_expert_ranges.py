@@ -1,0 +1,62 @@
+"""4-bit products at the ends of their types' ranges, against 64 bits. Tolerances as in test_gpu_experts, and where bf16 sums
+leave f32's normal numbers: the streaming kernels hold them 2^-15 times their value, so each of the (K / 32 + 16) additions is
+off by at most half of 2^-149, 2^-135 of the value, and the result by half a step of bf16's last digit, 2^-134. (Products and
+sums of activations are whole multiples of 2^-133 2^-15 = 2^-148 there, and exact.)"""
+import numpy as np
+import pytest
+
+import iree_b200 as ib
+from .test_gpu_experts import BF16, F16, Weights, product_tolerance, run_experts, run_matvec, to_bits, to_f64
+
+pytestmark = pytest.mark.gpu
+
+BF16_MAX = (2 - 2.0 ** -7) * 2.0 ** 127
+
+
+def scaled_weights(rng, kind, E, N, K, group, zeros, factor):
+    w = Weights(rng, kind, E, N, K, group, zeros)
+    before = to_f64(w.scales, kind)
+    w.scales = to_bits(before * factor, kind)
+    ratio = np.repeat(to_f64(w.scales, kind) / before, group, axis=-1)
+    w.w, w.magnitude = w.w * ratio, w.magnitude * ratio
+    return w
+
+
+def check_both(ctx, a64, w, group):
+    """The matrix-vector product and the streamed experts' product of one expert."""
+    M, K = a64.shape
+    a = to_bits(a64, BF16)
+    a64 = to_f64(a, BF16)
+    exact = a64 @ w.w[0].T
+    assert np.isfinite(exact).all() and (np.abs(exact) <= BF16_MAX).all()
+    tol = product_tolerance(a64, w.w[0], w.magnitude[0], exact, BF16, 2.0 ** -134 + (K / 32 + 16) * 2.0 ** -135)
+    got = to_f64(run_matvec(ctx, BF16, a, w, group), BF16)
+    assert (np.abs(got - exact) <= tol).all()
+    got = to_f64(run_experts(ctx, BF16, [M], M, w, group, a, ib.W4A16_EXPERTS_STREAM), BF16)
+    assert (np.abs(got - exact) <= tol).all()
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 64, 128])
+@pytest.mark.parametrize("M", [1, 12])
+def test_bf16_activations_near_the_largest(ctx, M, group, zeros):
+    """One activation of 3e36, and whole rows of the largest one: the sums that a result needs pass f32's range unscaled."""
+    rng = np.random.default_rng([M, group, int(zeros)])
+    K, N = 512, 70
+    w = scaled_weights(rng, BF16, 1, N, K, group, zeros, 2.0 ** -14)
+    a = rng.standard_normal((M, K))
+    a[0, 5] = 3e36
+    check_both(ctx, a, w, group)
+    check_both(ctx, np.full((M, K), BF16_MAX), w, group)
+    check_both(ctx, np.where(rng.random((M, K)) < 0.5, -BF16_MAX, BF16_MAX), w, group)
+
+
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("group", [32, 128])
+@pytest.mark.parametrize("scale", [2.0 ** -133, 2.0 ** -126, 2.0 ** -120, 2.0 ** -110])
+def test_bf16_activations_near_the_smallest(ctx, scale, group, zeros):
+    rng = np.random.default_rng([group, int(zeros)])
+    K, N = 256, 48
+    for factor in (1.0, 2.0 ** 10):
+        w = scaled_weights(rng, BF16, 1, N, K, group, zeros, factor)
+        check_both(ctx, rng.integers(-15, 16, (9, K)) * scale, w, group)
