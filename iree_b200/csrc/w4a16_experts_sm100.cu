@@ -505,10 +505,12 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
             if (c == 0 || per_pair == 4 || (per_pair == 2 && c == 2)) {
-              const uint32_t block = min(static_cast<uint32_t>(p) * 4 + c, last_block);
+              // behind K: scale and zero point 0, as (0 - z) s of the last group may be an infinity
+              const uint32_t block = static_cast<uint32_t>(p) * 4 + c;
               const uint32_t g = group_blocks > 1 ? __umulhi(block, magic) : block;
-              next_s[c] = s_row[g];
-              if (ZEROS) next_z[c] = z_row[g];
+              const bool there = block <= last_block;
+              next_s[c] = there ? s_row[g] : 0;
+              if (ZEROS) next_z[c] = there ? z_row[g] : 0;
             } else {
               next_s[c] = next_s[c - 1];
               next_z[c] = next_z[c - 1];

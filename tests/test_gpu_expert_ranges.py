@@ -6,7 +6,7 @@ import numpy as np
 import pytest
 
 import iree_b200 as ib
-from .test_gpu_experts import BF16, F16, Weights, product_tolerance, run_experts, run_matvec, to_bits, to_f64
+from .test_gpu_experts import BF16, F16, Weights, offsets_of, product_tolerance, run_experts, run_matvec, to_bits, to_f64
 
 pytestmark = pytest.mark.gpu
 
@@ -60,3 +60,26 @@ def test_bf16_activations_near_the_smallest(ctx, scale, group, zeros):
     for factor in (1.0, 2.0 ** 10):
         w = scaled_weights(rng, BF16, 1, N, K, group, zeros, factor)
         check_both(ctx, rng.integers(-15, 16, (9, K)) * scale, w, group)
+
+
+@pytest.mark.parametrize("variant", [ib.W4A16_EXPERTS_STREAM, ib.W4A16_EXPERTS_TENSOR])
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("K, group", [(32, 32), (160, 32), (224, 32), (192, 64), (288, 96)])
+@pytest.mark.parametrize("counts", [[5, 20], [150, 3]])
+def test_weights_that_do_not_exist_are_not_formed(ctx, counts, K, group, kind, variant):
+    """K that ends inside a chunk of 128: what stands behind it is stored nibble 0 by the reading, and 0 - zero point times the
+    last scale is an infinity here, while the weights that there are are -scale or 0. Whole numbers times one scale: exact."""
+    rng = np.random.default_rng([K, group, kind])
+    E, N, scale = len(counts), 40, 6000.0 if kind == F16 else 3e37
+    unit = 2.0 ** -6 if kind == F16 else 2.0 ** -30
+    w = Weights(rng, kind, E, N, K, group, True)
+    w.q = rng.integers(14, 16, (E, N, K))
+    w.wq = (w.q[..., 0::2] | (w.q[..., 1::2] << 4)).astype(np.uint8)
+    w.scales, w.zeros = to_bits(np.full(w.scales.shape, scale), kind), to_bits(np.full(w.scales.shape, 15.0), kind)
+    s = to_f64(w.scales, kind)[0, 0, 0]
+    a = rng.integers(-1, 2, (sum(counts), K)) * unit
+    got = run_experts(ctx, kind, counts, sum(counts), w, group, to_bits(a, kind), variant)
+    off = offsets_of(counts)
+    for e in range(E):
+        exact = a[off[e]:off[e + 1]] @ ((w.q[e] - 15) * s).T      # whole numbers up to 288, times one number of 11 bits
+        assert (got[off[e]:off[e + 1]] == to_bits(exact, kind)).all()
