@@ -228,9 +228,13 @@ uint64_t iree_hal_b200_command_buffer_launch_count(const iree_hal_b200_command_b
  * before the dispatch ahead of it has finished. Only exports that order themselves on the device
  * may be dispatched this way: they call griddepcontrol.wait before reading anything an earlier
  * kernel may write and before writing anything. Of this library's exports those are
- * b200_w4a16_decode_m8 / _m16, which prefetch weight tiles ahead of the wait: the caller vouches
- * that weights and scales are not written by the dispatch ahead. UNAVAILABLE when the driver
- * lacks the feature. */
+ * b200_w4a16_decode_m8 / _m16 and b200_w4a16_stream_*, which prefetch weights ahead of the wait:
+ * the caller vouches that weights, scales and zero points are not written by the dispatch ahead,
+ * nor, where that one is a contraction, W4A16, mmt4d or pack export launched early itself, by the
+ * ones ahead of it back to the last execution barrier: those exports release the next dispatch
+ * before they have waited. (The exports of the matrix-vector products and the expert layer
+ * release it afterwards: behind one of them only it can be unfinished.) UNAVAILABLE when the
+ * driver lacks the feature. */
 iree_b200_status_t iree_hal_b200_command_buffer_set_dispatch_overlap(iree_hal_b200_command_buffer_t* command_buffer,
                                                                      int32_t enable);
 
@@ -593,7 +597,7 @@ typedef struct {
 #define IREE_B200_MATVEC_MAX_ROWS 16
 /* out[M, N] = a[M, K] x w[N, K]^T, the weights read once. Needs no workspace. Under
  * iree_b200_context_set_dispatch_overlap the weights, scales and zeros are fetched before the dispatch ahead has finished, as
- * by the decode exports. */
+ * by the decode exports: see iree_hal_b200_command_buffer_set_dispatch_overlap for what may not be writing them. */
 iree_b200_status_t iree_b200_w4a16_matvec(iree_b200_context_t* context, const iree_b200_w4a16_matvec_params_t* params,
                                           const void* a, const void* wq, const void* scales, const void* zeros, void* out);
 

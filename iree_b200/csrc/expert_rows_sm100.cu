@@ -12,6 +12,9 @@
 // The sort counts. One CTA owns a run of tokens; what it has to know of the rest is how many slots go to each expert before
 // its run and in all. Up to 8192 slots every CTA counts all of them itself, one launch; above that a first launch leaves one
 // histogram per run and a second one sums them along the runs. Ranks inside a run come from warp votes.
+//
+// Every kernel here lets the next one on the stream start after its own wait, not before: a kernel further on that fetches weights
+// ahead of its wait (matrix-vector products under dispatch overlap) then finds only this one unfinished, not what it waited for.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
@@ -95,8 +98,8 @@ extern "C" __global__ void __launch_bounds__(b200::kRouteThreads)
     b200_expert_count(const int32_t* ids, int32_t* counts, int tokens, int slots, int experts, int first, int run) {
   __shared__ int hist[kRouteMaxExperts];
   for (int e = threadIdx.x; e < experts; e += kRouteThreads) hist[e] = 0;
-  grid_launch_dependents();
   grid_dependency_wait();
+  grid_launch_dependents();
   __syncthreads();
   const int64_t lo = static_cast<int64_t>(blockIdx.x) * run * slots;
   const int64_t hi = min(lo + static_cast<int64_t>(run) * slots, static_cast<int64_t>(tokens) * slots);
@@ -113,8 +116,8 @@ extern "C" __global__ void __launch_bounds__(b200::kRouteThreads)
 extern "C" __global__ void __launch_bounds__(b200::kRouteThreads)
     b200_expert_scan(int32_t* counts, int32_t* totals, int runs, int experts) {
   __shared__ int part_sum[kRouteWarps][32];
-  grid_launch_dependents();
   grid_dependency_wait();
+  grid_launch_dependents();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, e = blockIdx.x * 32 + lane;
   const int per = (runs + kRouteWarps - 1) / kRouteWarps, lo = warp * per, hi = min(lo + per, runs);
   constexpr int kBatch = 10;  // loads in flight per thread: all of a part, at most 148 runs / 16 warps
@@ -160,8 +163,8 @@ extern "C" __global__ void __launch_bounds__(b200::kRouteThreads)
   uint16_t* warp_count = reinterpret_cast<uint16_t*>(where + kRouteRun);  // [warp][expert], then slots of the warps before
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   for (int e = tid; e < experts; e += kRouteThreads) next[e] = total[e] = 0;
-  grid_launch_dependents();
   grid_dependency_wait();
+  grid_launch_dependents();
   __syncthreads();
   const int64_t all = static_cast<int64_t>(tokens) * slots;
   const int64_t t_lo = static_cast<int64_t>(blockIdx.x) * run, t_hi = min(t_lo + run, static_cast<int64_t>(tokens));
@@ -389,16 +392,16 @@ __device__ void combine_backward_body(const uint16_t* __restrict__ dout, const u
   extern "C" __global__ void __launch_bounds__(b200::kCombineThreads, 6)                                                   \
       b200_expert_combine_##SUFFIX(const uint16_t* rows, const float* weights, const int32_t* position, uint16_t* out,     \
                                    int tokens, int slots, int width, int ldr, int ldo, int row_count) {                    \
-    grid_launch_dependents();                                                                                              \
     grid_dependency_wait();                                                                                                \
+    grid_launch_dependents();                                                                                              \
     combine_body<BF16, 8, 2, 1>(rows, weights, position, out, tokens, slots, width, ldr, ldo, row_count);                     \
   }                                                                                                                        \
   extern "C" __global__ void __launch_bounds__(b200::kCombineThreads)                                                      \
       b200_expert_combine_narrow_##SUFFIX(const uint16_t* rows, const float* weights, const int32_t* position,             \
                                           uint16_t* out, int tokens, int slots, int width, int ldr, int ldo,               \
                                           int row_count, int vec) {                                                        \
-    grid_launch_dependents();                                                                                              \
     grid_dependency_wait();                                                                                                \
+    grid_launch_dependents();                                                                                              \
     if (vec == 4) combine_body<BF16, 4, 4, 2>(rows, weights, position, out, tokens, slots, width, ldr, ldo, row_count);       \
     else combine_body<BF16, 1, 2, 4>(rows, weights, position, out, tokens, slots, width, ldr, ldo, row_count);                \
   }                                                                                                                        \
@@ -406,8 +409,8 @@ __device__ void combine_backward_body(const uint16_t* __restrict__ dout, const u
       b200_expert_combine_backward_##SUFFIX(const uint16_t* dout, const uint16_t* rows, const float* weights,              \
                                             const int32_t* position, uint16_t* drows, float* dweights, int tokens,         \
                                             int slots, int width, int ldo, int ldr, int row_count, int vec) {              \
-    grid_launch_dependents();                                                                                              \
     grid_dependency_wait();                                                                                                \
+    grid_launch_dependents();                                                                                              \
     if (vec == 8)                                                                                                          \
       combine_backward_body<BF16, 8, 2>(dout, rows, weights, position, drows, dweights, tokens, slots, width, ldo, ldr,    \
                                         row_count);                                                                        \

@@ -174,7 +174,6 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
   static_assert(8 * (kNumRingBars + 3) <= kExBarrierBytes, "barrier area");
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  grid_launch_dependents();
   const int tiles_n = (N + kExWRows - 1) / kExWRows;
   const int num_kb = ((K + 127) >> 7) << 1;  // whole pairs of K blocks; TMA fills K behind the end with zeros
 
@@ -198,6 +197,7 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
     tmem_relinquish();
   }
   grid_dependency_wait();
+  grid_launch_dependents();  // behind the wait: whoever starts now finds no other kernel unfinished
   if (warp == 1) {  // the tile list: rows and tiles before each expert
     // A workspace that was not prepared for these operands holds no maps, or others': nothing is copied through it.
     const auto low = [](const void* p) { return static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p)); };

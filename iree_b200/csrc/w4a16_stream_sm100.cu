@@ -249,8 +249,13 @@ __device__ void stream_body(const StreamArgs& p) {
   const int last_block = (p.K >> 5) - 1;
   const int64_t w_pitch = p.K >> 1;
 
-  grid_launch_dependents();
-  if (p.offsets) grid_dependency_wait();
+  // The next kernel may start once this one has waited for those ahead: what it fetches before its own wait (weights, under
+  // dispatch overlap) can then be in the hands of this kernel only.
+  auto wait_for_dispatches_ahead = []() {
+    grid_dependency_wait();
+    grid_launch_dependents();
+  };
+  if (p.offsets) wait_for_dispatches_ahead();
   // Experts: how many passes (8 NB activation rows each) each one needs comes from the dispatch ahead.
   int64_t passes = (p.M + kCols - 1) / kCols;
   if (p.offsets) {
@@ -304,7 +309,7 @@ __device__ void stream_body(const StreamArgs& p) {
       else if (p.zeros) prefetch_l2(p.zeros + first * groups, groups * 2);
     }
   }
-  if (!p.offsets && !p.weights_ahead) grid_dependency_wait();
+  if (!p.offsets && !p.weights_ahead) wait_for_dispatches_ahead();
   const uint32_t mask = BF16 ? 0x000f000fu : 0x00f000f0u;
   const uint32_t under = BF16 ? (p.zeros ? 0x3b803b80u : 0x3b883b88u) : (p.zeros ? 0x54005400u : 0x54805480u);
   // what the unpacked nibbles stand above their values (bf16: in units of kStreamBf16Unit): of all of them, or without the zero
@@ -445,7 +450,7 @@ __device__ void stream_body(const StreamArgs& p) {
     issue_run();
 #pragma unroll
     for (int i = 0; i < kStreamRing; ++i) issue_unit();
-    if (!p.offsets && p.weights_ahead) grid_dependency_wait();  // weights and scales were fetched ahead, activations may not be
+    if (!p.offsets && p.weights_ahead) wait_for_dispatches_ahead();  // weights and scales were fetched ahead, activations may not be
     int turn = 0;  // which of the two batches is in use
     auto next_batch = [&](int into) {
       __syncwarp();  // every lane has read what was there
