@@ -367,40 +367,66 @@ class Context:
         check(library().iree_b200_w4a16_wait_arrivals(self.handle, _vp(own_flags), _vp(ws), C.c_int32(world),
                                                       C.c_int32(epoch)))
 
-    def _on_device(self, x, element_bytes: int, pitched: bool = False) -> int:
+    def _on_device(self, x, element_bytes: int, count: int, pitch: int = 1, width: int = 1) -> int:
         """Address of an array of the expert layer's calls: a torch tensor on this device with elements of that size, a
-        DeviceBuffer of this context, a device address, or None. Rows whose pitch the parameters give (``pitched``) need
-        adjacent elements, other tensors have no gaps at all."""
+        DeviceBuffer of this context, a device address, or None. The call reaches ``count`` elements from there on, in rows
+        of ``width`` that are ``pitch`` apart; a tensor holds those, in rows of that pitch."""
         if x is None:
             return 0
         try:
-            device = x.get_device()
+            if x.get_device() == self.ordinal and x.itemsize == element_bytes:
+                if pitch == width and x.numel() == count and x.is_contiguous():
+                    return x.data_ptr()
+                return self._with_layout(x, count, pitch, width)
         except AttributeError:
-            device = None
-        if device is not None:
-            if device != self.ordinal or x.itemsize != element_bytes:
-                raise IreeB200Error(3, "expected %d-byte elements on device %d, got %s on %s" % (element_bytes, self.ordinal,
-                                                                                             x.dtype, x.device))
-            if not x.is_contiguous() and not (pitched and x.dim() == 2 and x.stride(1) == 1):
-                raise IreeB200Error(3, "strides %s of a %s: its elements are not adjacent" % (x.stride(), tuple(x.shape)))
-            return x.data_ptr()
+            return self._not_a_tensor(x, element_bytes * count if width > 0 else 0)
+        raise IreeB200Error(3, "expected %d-byte elements on device %d, got %s on %s" % (element_bytes, self.ordinal, x.dtype,
+                                                                                     x.device))
+
+    def _not_a_tensor(self, x, nbytes: int) -> int:
         if isinstance(x, DeviceBuffer):
             if x.ctx.ordinal != self.ordinal:
                 raise IreeB200Error(3, "the buffer is on device %d, not %d" % (x.ctx.ordinal, self.ordinal))
+            if x.nbytes < nbytes:
+                raise IreeB200Error(3, "a buffer of %d bytes where the parameters say %d" % (x.nbytes, nbytes))
             return x.ptr
         if isinstance(x, int):
             return x
         raise IreeB200Error(3, "expected a device array, got %s" % type(x).__name__)
 
-    def _scratch(self, x) -> int:
-        return self._on_device(x, x.element_size()) if hasattr(x, "element_size") else self._on_device(x, 1)
+    def _with_layout(self, x, count: int, pitch: int, width: int) -> int:
+        """A tensor that is not just ``count`` elements without gaps: larger than that, or rows with a pitch of their own."""
+        if pitch <= 0 or width <= 0:
+            return x.data_ptr()  # the call refuses these parameters, or touches nothing
+        shape, strides, rows = tuple(x.shape), x.stride(), (count - width) // pitch + 1
+        if x.is_contiguous():  # any split of a row over dimensions
+            if x.numel() >= count and (rows <= 1 or len(shape) < 2 or pitch in strides[:-1]):
+                return x.data_ptr()
+        elif len(shape) != 2 or strides[1] != 1:
+            raise IreeB200Error(3, "strides %s of a %s: its elements are not adjacent" % (strides, shape))
+        elif shape[0] >= rows and shape[1] >= width and (rows <= 1 or strides[0] == pitch):
+            return x.data_ptr()
+        raise IreeB200Error(3, "a %s with strides %s where the parameters say %d rows of %d, %d elements apart" % (
+            shape, strides, rows, width, pitch))
+
+    def _scratch(self, x, nbytes: int) -> int:
+        if hasattr(x, "element_size"):
+            return self._on_device(x, x.element_size(), -(-nbytes // x.element_size()))
+        return self._on_device(x, 1, nbytes)
 
     # 4-bit matrix-vector products and the expert layer. Arrays: torch tensors on this device, DeviceBuffers or addresses.
     def w4a16_matvec(self, params: W4A16MatvecParams, a, wq, scales, zeros, out) -> None:
         """out[M, N] = a[M, K] x w[N, K]^T for up to 16 rows; ``zeros`` None: signed weights."""
+        M, N, K, lda, ldo, at = params.M, params.N, params.K, params.lda, params.ldo, self._on_device
+        G = K // (params.group_size or 1)
         check(library().iree_b200_w4a16_matvec(
-            self.handle, C.addressof(params), self._on_device(a, 2, True), self._on_device(wq, 1),
-            self._on_device(scales, 2), self._on_device(zeros, 2), self._on_device(out, 2, True)))
+            self.handle, C.addressof(params), at(a, 2, (M - 1) * lda + K, lda, K), at(wq, 1, N * K // 2, K // 2, K // 2),
+            at(scales, 2, N * G, G, G), at(zeros, 2, N * G, G, G), at(out, 2, (M - 1) * ldo + N, ldo, N)))
+
+    def _experts_arrays(self, p: W4A16ExpertsParams, a, wq, out):
+        rows, N, K, lda, ldo, at = p.rows, p.N, p.K, p.lda, p.ldo, self._on_device
+        return (at(a, 2, (rows - 1) * lda + K, lda, K), at(wq, 1, p.experts * N * K // 2, K // 2, K // 2),
+                at(out, 2, (rows - 1) * ldo + N, ldo, N))
 
     def w4a16_experts_workspace(self, params: W4A16ExpertsParams) -> DeviceBuffer:
         nbytes = int(library().iree_b200_w4a16_experts_workspace_bytes(C.byref(params)))
@@ -408,22 +434,29 @@ class Context:
 
     def w4a16_experts_prepare(self, params: W4A16ExpertsParams, a, wq, out, ws) -> int:
         variant = C.c_int32()
+        a, wq, out = self._experts_arrays(params, a, wq, out)
         check(library().iree_b200_w4a16_experts_prepare(
-            self.handle, C.byref(params), C.c_void_p(self._on_device(a, 2, True)), C.c_void_p(self._on_device(wq, 1)),
-            C.c_void_p(self._on_device(out, 2, True)), C.c_void_p(self._scratch(ws)), C.byref(variant)))
+            self.handle, C.byref(params), C.c_void_p(a), C.c_void_p(wq), C.c_void_p(out),
+            C.c_void_p(self._scratch(ws, WORKSPACE_BYTES)), C.byref(variant)))
         return variant.value
 
     def w4a16_experts_run(self, params: W4A16ExpertsParams, a, wq, scales, zeros, offsets, out, ws, variant: int) -> None:
+        E, at = params.experts, self._on_device
+        a, wq, out = self._experts_arrays(params, a, wq, out)
+        G = params.K // (params.group_size or 1)
+        groups = E * params.N * G
         check(library().iree_b200_w4a16_experts_run(
-            self.handle, C.addressof(params), self._on_device(a, 2, True), self._on_device(wq, 1),
-            self._on_device(scales, 2), self._on_device(zeros, 2), self._on_device(offsets, 4),
-            self._on_device(out, 2, True), self._scratch(ws), variant))
+            self.handle, C.addressof(params), a, wq, at(scales, 2, groups, G, G), at(zeros, 2, groups, G, G),
+            at(offsets, 4, E + 1), out, self._scratch(ws, WORKSPACE_BYTES), variant))
 
     def w4a16_experts(self, params: W4A16ExpertsParams, a, wq, scales, zeros, offsets, out, ws) -> None:
+        E, at = params.experts, self._on_device
+        a, wq, out = self._experts_arrays(params, a, wq, out)
+        G = params.K // (params.group_size or 1)
+        groups = E * params.N * G
         check(library().iree_b200_w4a16_experts(
-            self.handle, C.addressof(params), self._on_device(a, 2, True), self._on_device(wq, 1),
-            self._on_device(scales, 2), self._on_device(zeros, 2), self._on_device(offsets, 4),
-            self._on_device(out, 2, True), self._scratch(ws)))
+            self.handle, C.addressof(params), a, wq, at(scales, 2, groups, G, G), at(zeros, 2, groups, G, G),
+            at(offsets, 4, E + 1), out, self._scratch(ws, WORKSPACE_BYTES)))
 
     def expert_dispatch_workspace(self, params: ExpertRowsParams) -> Optional[DeviceBuffer]:
         """None where the dispatch needs none."""
@@ -432,27 +465,37 @@ class Context:
 
     def expert_dispatch(self, params: ExpertRowsParams, expert_ids, x, offsets, position, order, rows, ws) -> None:
         """Sorts (token, slot) pairs by expert and copies the tokens' rows there."""
+        T, k, D, tp, rp, at = params.tokens, params.slots, params.width, params.token_pitch, params.row_pitch, self._on_device
+        P = T * k
+        if ws is not None:
+            ws = self._scratch(ws, library().iree_b200_expert_dispatch_workspace_bytes(C.byref(params)))
         check(library().iree_b200_expert_dispatch(
-            self.handle, C.addressof(params), self._on_device(expert_ids, 4), self._on_device(x, 2, True),
-            self._on_device(offsets, 4), self._on_device(position, 4), self._on_device(order, 4),
-            self._on_device(rows, 2, True), self._scratch(ws)))
+            self.handle, C.addressof(params), at(expert_ids, 4, P, k, k), at(x, 2, (T - 1) * tp + D, tp, D),
+            at(offsets, 4, params.experts + 1), at(position, 4, P, k, k), at(order, 4, P),
+            at(rows, 2, (P - 1) * rp + D, rp, D), ws))
 
     def expert_dispatch_backward(self, params: ExpertRowsParams, drows, position, dx) -> None:
+        T, k, D, tp, rp, at = params.tokens, params.slots, params.width, params.token_pitch, params.row_pitch, self._on_device
+        P = T * k
         check(library().iree_b200_expert_dispatch_backward(
-            self.handle, C.addressof(params), self._on_device(drows, 2, True), self._on_device(position, 4),
-            self._on_device(dx, 2, True)))
+            self.handle, C.addressof(params), at(drows, 2, (P - 1) * rp + D, rp, D), at(position, 4, P, k, k),
+            at(dx, 2, (T - 1) * tp + D, tp, D)))
 
     def expert_combine(self, params: ExpertRowsParams, rows, weights, position, out) -> None:
         """out[t] = sum of weights[t, j] * rows[position[t, j]]."""
+        T, k, D, tp, rp, at = params.tokens, params.slots, params.width, params.token_pitch, params.row_pitch, self._on_device
+        P = T * k
         check(library().iree_b200_expert_combine(
-            self.handle, C.addressof(params), self._on_device(rows, 2, True), self._on_device(weights, 4),
-            self._on_device(position, 4), self._on_device(out, 2, True)))
+            self.handle, C.addressof(params), at(rows, 2, (P - 1) * rp + D, rp, D), at(weights, 4, P, k, k),
+            at(position, 4, P, k, k), at(out, 2, (T - 1) * tp + D, tp, D)))
 
     def expert_combine_backward(self, params: ExpertRowsParams, dout, rows, weights, position, drows, dweights) -> None:
+        T, k, D, tp, rp, at = params.tokens, params.slots, params.width, params.token_pitch, params.row_pitch, self._on_device
+        P = T * k
+        n = (P - 1) * rp + D
         check(library().iree_b200_expert_combine_backward(
-            self.handle, C.addressof(params), self._on_device(dout, 2, True), self._on_device(rows, 2, True),
-            self._on_device(weights, 4), self._on_device(position, 4), self._on_device(drows, 2, True),
-            self._on_device(dweights, 4)))
+            self.handle, C.addressof(params), at(dout, 2, (T - 1) * tp + D, tp, D), at(rows, 2, n, rp, D), at(weights, 4, P, k, k),
+            at(position, 4, P, k, k), at(drows, 2, n, rp, D), at(dweights, 4, P, k, k)))
 
     def w4a16_host(self, params: W4A16Params, a, wq, scales, out) -> None:
         check(library().iree_b200_w4a16_host(self.handle, C.byref(params), _vp(a), _vp(wq), _vp(scales), _vp(out)))
