@@ -84,6 +84,12 @@ iree_b200_status_t iree_hal_b200_device_query(iree_hal_b200_device_t* device, ch
 iree_b200_status_t iree_hal_b200_device_synchronize(iree_hal_b200_device_t* device);
 /* The dispatch CUstream, for callers that interleave their own work (graph capture, NCCL). */
 void* iree_hal_b200_device_stream(iree_hal_b200_device_t* device);
+/* Makes a CUstream of the caller's the dispatch stream (the legacy default stream is CU_STREAM_LEGACY, 1), NULL the device's own
+ * again: what is queued through the device from then on runs behind the work queued so far on the stream before, and in order
+ * with the caller's own work on that stream. A program whose buffers another library writes, reads and recycles on one stream
+ * (torch's allocator hands memory out again in stream order) hands that stream over instead of synchronising around every call.
+ * The stream has to live until the device is released or given another one. */
+iree_b200_status_t iree_hal_b200_device_set_stream(iree_hal_b200_device_t* device, void* stream);
 
 /* ---- timing events --------------------------------------------------------------------------
  * CUevent pairs recorded on the dispatch stream, what the driver's tracing context wraps around

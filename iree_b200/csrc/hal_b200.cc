@@ -426,7 +426,8 @@ size_t align_up(std::vector<uint8_t>& b, size_t a) {
 struct iree_hal_b200_device_t {
   CUdevice device = 0;
   CUcontext context = nullptr;
-  CUstream stream = nullptr;
+  CUstream stream = nullptr;      // the dispatch stream: the device's own, or the caller's (set_stream)
+  CUstream own_stream = nullptr;
   // Second stream for collectives that may overlap later dispatches, with the two events that
   // order it against the dispatch stream (created on first use).
   CUstream collective_stream = nullptr;
@@ -547,7 +548,8 @@ iree_b200_status_t iree_hal_b200_device_create(int32_t ordinal, iree_hal_b200_de
     return st;
   }
   st = cu_check(g_cu.cuCtxSetCurrent(d->context), "cuCtxSetCurrent");
-  if (!st) st = cu_check(g_cu.cuStreamCreate(&d->stream, CU_STREAM_NON_BLOCKING), "cuStreamCreate");
+  if (!st) st = cu_check(g_cu.cuStreamCreate(&d->own_stream, CU_STREAM_NON_BLOCKING), "cuStreamCreate");
+  d->stream = d->own_stream;
   int major = 0, minor = 0;
   if (!st) {
     g_cu.cuDeviceGetName(d->name, sizeof d->name, d->device);
@@ -593,9 +595,10 @@ void iree_hal_b200_device_release(iree_hal_b200_device_t* device) {
     g_cu.cuStreamDestroy(device->upload_stream);
     g_cu.cuEventDestroy(device->upload_ready);
   }
-  if (device->stream) {
-    g_cu.cuStreamSynchronize(device->stream);
-    g_cu.cuStreamDestroy(device->stream);
+  if (device->own_stream) {
+    if (device->stream != device->own_stream) g_cu.cuStreamSynchronize(device->stream);
+    g_cu.cuStreamSynchronize(device->own_stream);
+    g_cu.cuStreamDestroy(device->own_stream);
   }
   g_cu.cuDevicePrimaryCtxRelease(device->device);
   delete device;
@@ -620,6 +623,20 @@ iree_b200_status_t iree_hal_b200_device_synchronize(iree_hal_b200_device_t* devi
 }
 
 void* iree_hal_b200_device_stream(iree_hal_b200_device_t* device) { return device ? device->stream : nullptr; }
+
+iree_b200_status_t iree_hal_b200_device_set_stream(iree_hal_b200_device_t* device, void* stream) {
+  if (!device) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "device is NULL");
+  const CUstream next = stream ? static_cast<CUstream>(stream) : device->own_stream;
+  if (next == device->stream) return IREE_B200_STATUS_OK;
+  CU_RETURN_IF_ERROR(g_cu.cuCtxSetCurrent(device->context), "cuCtxSetCurrent");
+  CUevent event = nullptr;
+  CU_RETURN_IF_ERROR(g_cu.cuEventCreate(&event, CU_EVENT_DISABLE_TIMING), "cuEventCreate");
+  iree_b200_status_t st = cu_check(g_cu.cuEventRecord(event, device->stream), "cuEventRecord");
+  if (!st) st = cu_check(g_cu.cuStreamWaitEvent(next, event, 0), "cuStreamWaitEvent");
+  g_cu.cuEventDestroy(event);
+  if (!st) device->stream = next;
+  return st;
+}
 
 // ---- events ----------------------------------------------------------------------------------
 iree_b200_status_t iree_hal_b200_event_create(iree_hal_b200_device_t* device, void** out_event) {

@@ -234,6 +234,13 @@ class Context:
     def stream(self) -> int:
         return library().iree_hal_b200_device_stream(self.device) or 0
 
+    def set_stream(self, stream) -> None:
+        """Queues this context's work on ``stream`` from now on, behind what it has queued so far: a ``torch.cuda.Stream``, a
+        CUstream handle (0: the legacy default stream), or None for the context's own. On torch's current stream the calls are
+        in order with torch's work on their tensors, and memory that torch hands out again is not still in use here."""
+        handle = getattr(stream, "cuda_stream", stream)
+        check(library().iree_hal_b200_device_set_stream(self.device, C.c_void_p(None if handle is None else handle or 1)))
+
     @property
     def launch_count(self) -> int:
         return int(library().iree_hal_b200_command_buffer_launch_count(self.command_buffer))
@@ -414,7 +421,8 @@ class Context:
             return self._on_device(x, x.element_size(), -(-nbytes // x.element_size()))
         return self._on_device(x, 1, nbytes)
 
-    # 4-bit matrix-vector products and the expert layer. Arrays: torch tensors on this device, DeviceBuffers or addresses.
+    # 4-bit matrix-vector products and the expert layer. Arrays: torch tensors on this device, DeviceBuffers or addresses. Torch's
+    # streams do not wait for the context's, nor it for them, unless they are the same one (set_stream).
     def w4a16_matvec(self, params: W4A16MatvecParams, a, wq, scales, zeros, out) -> None:
         """out[M, N] = a[M, K] x w[N, K]^T for up to 16 rows; ``zeros`` None: signed weights."""
         M, N, K, lda, ldo, at = params.M, params.N, params.K, params.lda, params.ldo, self._on_device
