@@ -237,18 +237,24 @@ _PLAIN = dict(matvec=_plain_matvec, dispatch=_plain_dispatch, experts=_plain_exp
 
 
 def _context():
+    """One per device and stream: its work is queued on torch's current stream, in order with whoever makes the inputs and
+    reads the results."""
     import iree_b200
-    device = torch.cuda.current_device()
-    if device not in _contexts:
-        _contexts[device] = iree_b200.Context(device)
-    return _contexts[device]
+    device, stream = torch.cuda.current_device(), torch.cuda.current_stream()
+    key = device, stream.cuda_stream
+    if key not in _contexts:
+        _contexts[key] = iree_b200.Context(device)
+        _contexts[key].set_stream(stream)
+    return _contexts[key]
 
 
 def _run_own(s):
-    """The calls of a program that keeps its parameter blocks, workspaces and (experts) prepared maps from call to call;
-    they are made on a state's first pass."""
+    """The calls of a program that keeps its context, parameter blocks, workspaces and (experts) prepared maps from call to
+    call; they are made on a state's first pass, for the stream that is current then."""
     import iree_b200 as ib
-    ctx, case, op = _context(), s["case"], s["op"]
+    if "ctx" not in s:
+        s["ctx"] = _context()
+    ctx, case, op = s["ctx"], s["case"], s["op"]
     kind = ib.KIND_F16 if case["type"] == "f16" else ib.KIND_BF16
     if op == "matvec":
         if "p" not in s:
