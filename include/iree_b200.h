@@ -590,7 +590,8 @@ int32_t iree_b200_w4a16_host_plan(const iree_b200_w4a16_params_t* params, int32_
  * no result depends on other rows or on the memory behind the last one. Every finite activation is good for every finite result
  * (zero points up to 128 in magnitude); the streaming kernels hold bf16 sums at 2^-15 of their value, so that results below 2^-111
  * carry an absolute error of up to (K / 32 + 16) 2^-135 beside their rounding. Every call queues work on the context's stream and returns; it may
- * be recorded into a graph (begin_graph); calls share no scratch but the workspace they are given. All pointers are device
+ * be recorded into a graph (begin_graph); calls share no scratch but the workspace they are given. A result may
+ * overlap no operand. All pointers are device
  * pointers: wq on a 16-byte, scales / zeros / activations / results on a 2-byte, index and f32 arrays on a 4-byte boundary
  * (INVALID_ARGUMENT otherwise). Activations, rows and results on 16-byte boundaries with pitches of whole 16-byte pieces
  * take the fast paths; others are right and slower. */
@@ -623,7 +624,7 @@ typedef struct {
  *   offsets[experts + 1]      rows of the experts before each one; offsets[experts] = rows in all
  *   position[tokens, slots]   the slot's row, -1 for a dropped slot
  *   order[tokens * slots]     token * slots + slot of each row, -1 behind the last row
- *   rows[position[t, j]]      = x[t]; rows behind the last one are left as they were
+ *   rows[position[t, j]]      = x[t]; rows behind the last one are left as they were. rows may not overlap x
  * An id may occur twice in one token: both slots get a row. `workspace` has
  * iree_b200_expert_dispatch_workspace_bytes(params) bytes (0: NULL will do), 4-byte aligned, need not be initialised and
  * holds nothing after the call. */
@@ -631,7 +632,8 @@ size_t iree_b200_expert_dispatch_workspace_bytes(const iree_b200_expert_rows_par
 iree_b200_status_t iree_b200_expert_dispatch(iree_b200_context_t* context, const iree_b200_expert_rows_params_t* params,
                                              const int32_t* expert_ids, const void* x, int32_t* offsets, int32_t* position,
                                              int32_t* order, void* rows, void* workspace);
-/* Its gradient: dx[t] = sum over the token's slots of drows[position[t, j]] (a token whose slots were all dropped: zeros). */
+/* Its gradient: dx[t] = sum over the token's slots of drows[position[t, j]] (a token whose slots were all dropped: zeros). dx may
+ * not overlap drows. */
 iree_b200_status_t iree_b200_expert_dispatch_backward(iree_b200_context_t* context,
                                                       const iree_b200_expert_rows_params_t* params, const void* drows,
                                                       const int32_t* position, void* dx);

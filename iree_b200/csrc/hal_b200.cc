@@ -19,6 +19,7 @@
 #include <mutex>
 #include <string>
 #include <thread>
+#include <utility>
 #include <vector>
 
 #include "../../include/iree_b200.h"
@@ -2749,6 +2750,27 @@ static iree_b200_status_t rows_check(const void* a, const void* b, const void* c
   return IREE_B200_STATUS_OK;
 }
 
+// Whether two arrays of 16-bit rows of `width` share an element, as far as pitches tell: both without gaps, or of one pitch
+// (columns side by side in one buffer share none). Other pairs are taken not to.
+static bool rows_overlap(const void* a, int64_t rows_a, int64_t pitch_a, const void* b, int64_t rows_b, int64_t pitch_b,
+                         int64_t width) {
+  if (!a || !b || rows_a <= 0 || rows_b <= 0 || width <= 0) return false;
+  uint64_t low = reinterpret_cast<uintptr_t>(a), high = reinterpret_cast<uintptr_t>(b);
+  if (low > high) {
+    std::swap(low, high);
+    std::swap(rows_a, rows_b);
+    std::swap(pitch_a, pitch_b);
+  }
+  const int64_t bytes = 2 * width, pitch = 2 * pitch_a, apart = static_cast<int64_t>(high - low);
+  if (apart >= (rows_a - 1) * pitch + bytes) return false;
+  const bool dense_a = rows_a == 1 || pitch_a == width, dense_b = rows_b == 1 || pitch_b == width;
+  if (apart < bytes || (dense_a && dense_b)) return true;
+  if (pitch_a != pitch_b && rows_b > 1) return false;
+  // high's first row starts in row `row` of low's, `into` bytes behind its start
+  const int64_t row = apart / pitch, into = apart % pitch;
+  return into < bytes || (row + 1 < rows_a && into + bytes > pitch);
+}
+
 // Runs of tokens (grid x) and column parts (grid y) of the routing kernel: one CTA per SM over the runs, and
 // where there are few tokens their rows cut into parts.
 static void route_grid(const iree_b200_expert_rows_params_t* p, int sms, int* run, int* runs, int* part_width, int* parts) {
@@ -2782,6 +2804,8 @@ iree_b200_status_t iree_b200_expert_dispatch(iree_b200_context_t* context, const
   B200_RETURN_IF_ERROR(rows_check(nullptr, nullptr, nullptr, order, workspace, nullptr));
   const bool counted = static_cast<int64_t>(p.tokens) * p.slots > kRouteSingleSlots;
   if (counted && !workspace) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "workspace is NULL");
+  if (rows_overlap(x, p.tokens, p.token_pitch, rows, static_cast<int64_t>(p.tokens) * p.slots, p.row_pitch, p.width))
+    return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "the rows may not overlap the tokens'");
   if (!context) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "context is NULL");
   int sms = usable_sms(context);
   if (sms > 148) sms = 148;
@@ -2806,7 +2830,8 @@ static iree_b200_status_t combine_dispatch(iree_b200_context_t* context, const i
                                            const void* rows, const float* weights, const int32_t* position, void* out) {
   const bool empty = !p.tokens || !p.width;
   if (!empty && (!rows || !position || !out)) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "operand pointer is NULL");
-  if (!empty && rows == out) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "the result may not overlap the rows");
+  if (!empty && rows_overlap(out, p.tokens, p.token_pitch, rows, static_cast<int64_t>(p.tokens) * p.slots, p.row_pitch, p.width))
+    return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "the result may not overlap the rows");
   B200_RETURN_IF_ERROR(rows_check(rows, out, nullptr, weights, position, nullptr));
   if (!context) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "context is NULL");
   if (empty) return IREE_B200_STATUS_OK;
@@ -2844,7 +2869,9 @@ iree_b200_status_t iree_b200_expert_combine_backward(iree_b200_context_t* contex
   const auto& p = *params;
   if (p.tokens && (!weights || !position || !dweights || (p.width && (!dout || !rows || !drows))))
     return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "operand pointer is NULL");
-  if (p.tokens && p.width && (drows == rows || drows == dout))
+  const int64_t slots = static_cast<int64_t>(p.tokens) * p.slots;
+  if (rows_overlap(drows, slots, p.row_pitch, rows, slots, p.row_pitch, p.width) ||
+      rows_overlap(drows, slots, p.row_pitch, dout, p.tokens, p.token_pitch, p.width))
     return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "drows may not overlap rows or dout");
   B200_RETURN_IF_ERROR(rows_check(dout, rows, drows, weights, position, dweights));
   if (!context) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "context is NULL");

@@ -122,9 +122,12 @@ def test_what_is_larger_or_cut_otherwise_is_taken(ctx):
 
 
 def test_device_buffers_hold_what_the_parameters_say(ctx):
+    made = []
+
     def buffer(nbytes):
         b = ib.DeviceBuffer.__new__(ib.DeviceBuffer)
-        b.ctx, b.nbytes, b.ptr = ctx, nbytes, 1 << 20
+        b.ctx, b.nbytes, b.ptr = ctx, nbytes, (len(made) + 1) << 20
+        made.append(b)
         return b
 
     M, N, K = 2, 8, 64
