@@ -14,7 +14,8 @@
 // What differs: tiles are (expert, 128 weight rows, up to 256 activation rows), listed from the device's row offsets by every
 // CTA itself. An expert's rows are cut into equal parts of a multiple of 16 (260 rows are 2 x 144, not 256 + 16), and the
 // instruction is only as wide as the part. Rows of the next expert that a box brings along fall into accumulator columns
-// that are not read; a piece of 64 result rows that the expert does not fill is stored by the threads, others by TMA.
+// that are not read; a piece of 64 result rows that the expert does not fill, or whose last columns are a part of 16 bytes, is
+// stored by the threads, others by TMA.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <stdint.h>
@@ -380,7 +381,7 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
       __syncwarp();
     }
   } else if (warp >= 4 && warp < 8) {
-    // -------- epilogue: D[n, i] -> staged [i, n] pieces -> TMA stores, or the threads' own for a part piece ----
+    // -------- epilogue: D[n, i] -> staged [i, n] pieces -> TMA stores, or the threads' own ---------------------
     const int qd = warp & 3, et = threadIdx.x - 128;
     const bool issuer = et == 0;
     if (issuer) tensormap_fence_acquire(ws->map_out);
@@ -426,8 +427,9 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
         }
         fence_proxy_async_smem();
         named_barrier_sync(1, 128);
-        const int left = x.rows - pc * kExOutRows, y = x.row0 + pc * kExOutRows;
-        if (left >= kExOutRows) {
+        const int left = min(x.rows - pc * kExOutRows, kExOutRows), y = x.row0 + pc * kExOutRows;
+        // A TMA store writes whole 16-byte pieces: where N ends inside one, it would write behind N as well.
+        if (left == kExOutRows && (N % 8 == 0 || x.n0 + kExWRows <= N)) {
           if (issuer) tma_store_2d(ws->map_out, stage, x.n0, y);
         } else {
           for (int i = et; i < left * (kExWRows / 8); i += 128) {
@@ -444,7 +446,7 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
             }
           }
         }
-        if (issuer) bulk_commit_group();  // one group per piece, empty for a part piece
+        if (issuer) bulk_commit_group();  // one group per piece, empty where the threads store
         ++piece_it;
       }
     }
