@@ -450,10 +450,10 @@ class RewriteContractionsPass : public PassWrapper<RewriteContractionsPass, Oper
       m.last->getResult(0).replaceAllUsesWith(ext->getResult(0));
       return success();
     }
-    if ((ldo * 2) % 16 == 0 && nOff % 8 == 0) {
+    if ((ldo * 2) % 16 == 0 && nOff % 8 == 0 && N % 8 == 0) {
       // more than sixteen rows: weights as the tensor-memory operand; 128 weight rows x 128 (M <= 128) or 256
       // activation rows per tile; results leave by TMA stores through the output map at byte 512 of the
-      // workspace (one destination), which needs the result's pitch and offset on 16-byte boundaries
+      // workspace (one destination), which needs the result's pitch, offset and width in whole 16-byte pieces
       Value ws = workspace(b, loc, 512 + 8 * 128 + 8 * 8);
       ws = encodeMap(b, loc, m.activations, table, ws, 0, kF16Sw128R3, 3, {K, M, 1}, {K * 2, M * K * 2}, {64, 128, 1}, 2, 1);
       ws = encodeMap(b, loc, m.weights, table, ws, 128, kU8Sw64R3, 3, {K / 2, N, 1}, {K / 2, N * (K / 2)}, {64, 128, 1}, 1, 0);

@@ -2901,9 +2901,10 @@ static int w4_variant(const iree_b200_context_t* ctx, const iree_b200_w4a16_para
   if (p->group_size == 128 && aligned && p->K % 128 == 0) {
     // The kernel with the weights as the tensor-memory operand (activation tiles of 128 rows up to
     // M = 128, of 256 above); it leaves its results by TMA stores, which need the result on 16-byte
-    // boundaries. Otherwise the kernel with the expanded weights as a shared-memory operand.
+    // boundaries and write whole 16-byte pieces. Otherwise the kernel with the expanded weights as a
+    // shared-memory operand.
     const bool out16 = !(reinterpret_cast<uintptr_t>(out) % 16) && (static_cast<int64_t>(p->ldo) * 2) % 16 == 0 &&
-                       p->n_offset % 8 == 0;
+                       p->n_offset % 8 == 0 && p->N % 8 == 0;
     return out16 ? IREE_B200_W4A16_GEMM_WT : IREE_B200_W4A16_GEMM;
   }
   return IREE_B200_W4A16_GENERIC;
@@ -3003,8 +3004,9 @@ static iree_b200_status_t w4_encode_wt(const iree_b200_w4a16_params_t* params, c
                                        uint8_t host[kWtWorkspaceBytes]) {
   if (world < 1 || world > kWtMaxDestinations)
     return fail(IREE_B200_STATUS_OUT_OF_RANGE, "1 to %d destinations", kWtMaxDestinations);
-  if (params->n_offset % 8)
-    return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "n_offset must be a multiple of 8 (TMA stores start on 16-byte boundaries)");
+  if (params->n_offset % 8 || params->N % 8)
+    return fail(IREE_B200_STATUS_INVALID_ARGUMENT,
+                "n_offset and N must be multiples of 8 (TMA stores start on 16-byte boundaries and write whole 16-byte pieces)");
   memset(host, 0, kWtWorkspaceBytes);
   B200_RETURN_IF_ERROR(encode_map(CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, CU_TENSOR_MAP_SWIZZLE_128B, 128, a, params->K,
                                   params->M, 1, 64, 128, host));
@@ -3108,8 +3110,9 @@ static iree_b200_status_t w4_run_wt(iree_b200_context_t* context, const iree_b20
                                     const void* scales, void* out, void* workspace, int32_t world, int32_t rank,
                                     int32_t epoch) {
   if (!workspace) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "workspace is NULL");
-  if (params->group_size != 128 || params->K % 128 || params->n_offset % 8)
-    return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "this kernel needs group size 128, K %% 128 == 0 and n_offset %% 8 == 0");
+  if (params->group_size != 128 || params->K % 128 || params->n_offset % 8 || params->N % 8)
+    return fail(IREE_B200_STATUS_INVALID_ARGUMENT,
+                "this kernel needs group size 128, K %% 128 == 0, N %% 8 == 0 and n_offset %% 8 == 0");
   auto* cb = context->command_buffer;
   iree_hal_b200_descriptor_set_binding_t bindings[3] = {{0, const_cast<void*>(scales)}, {1, out}, {2, workspace}};
   const int32_t constants[7] = {params->M, params->N, params->K, params->ldo, params->n_offset, (world << 8) | rank, epoch};
