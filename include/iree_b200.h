@@ -585,16 +585,19 @@ int32_t iree_b200_w4a16_host_plan(const iree_b200_w4a16_params_t* params, int32_
  *   w[n, k] = q[n, k] * scales[n, k / group]                           zeros NULL: q is two's complement, -8..7
  *
  * wq is [N, K/2] bytes (element 2i in the low nibble of byte i, as for iree_b200_w4a16), scales and zeros are [N, K/group]
- * in the kind's type. Sums are f32 and the result is rounded once. A row of activations that
- * is not finite gives results that are not (the streaming kernels: NaN where the exact sum is an infinity), and only that row:
- * no result depends on other rows or on the memory behind the last one. Every finite activation is good for every finite result
- * (zero points up to 128 in magnitude); the streaming kernels hold bf16 sums at 2^-15 of their value, so that results below 2^-111
- * carry an absolute error of up to (K / 32 + 16) 2^-135 beside their rounding. Every call queues work on the context's stream and returns; it may
- * be recorded into a graph (begin_graph); calls share no scratch but the workspace they are given. A result may
- * overlap no operand. All pointers are device
- * pointers: wq on a 16-byte, scales / zeros / activations / results on a 2-byte, index and f32 arrays on a 4-byte boundary
- * (INVALID_ARGUMENT otherwise). Activations, rows and results on 16-byte boundaries with pitches of whole 16-byte pieces
- * take the fast paths; others are right and slower. */
+ * in the kind's type. Sums are f32 and the result is rounded once; the tensor-core variant of the experts' products (TENSOR
+ * below, which AUTO may pick) rounds the weights to the kind's type as well.
+ *
+ * A row of activations that is not finite gives results that are not (the streaming kernels: NaN where the exact sum is an
+ * infinity), and only that row: no result depends on other rows or on the memory behind the last one. The streaming kernels take
+ * every finite activation, with zero points up to 128 in magnitude; they hold bf16 sums at 2^-15 of their value, so that results
+ * below 2^-111 carry an absolute error of up to (K / 32 + 16) 2^-135 beside their rounding.
+ *
+ * Every call queues work on the context's stream and returns; it may be recorded into a graph (begin_graph); calls share no
+ * scratch but the workspace they are given. A result may overlap no operand. All pointers are device pointers: wq on a 16-byte,
+ * scales / zeros / activations / results on a 2-byte, index and f32 arrays on a 4-byte boundary (INVALID_ARGUMENT otherwise).
+ * Activations, rows and results on 16-byte boundaries with pitches of whole 16-byte pieces take the fast paths; others are right
+ * and slower. */
 typedef struct {
   int32_t kind;       /* IREE_B200_KIND_F16 or IREE_B200_KIND_BF16: activations, scales, zeros, result */
   int32_t M, N, K;    /* 0 <= M <= IREE_B200_MATVEC_MAX_ROWS */
@@ -658,7 +661,11 @@ enum {
                                          result */
   IREE_B200_W4A16_EXPERTS_TENSOR = 2, /* tcgen05 tiles of 128 weight rows x up to 256 rows; a and out on 16-byte boundaries,
                                          lda and ldo multiples of 8, experts * N < 2^31 (INVALID_ARGUMENT otherwise; AUTO then
-                                         picks STREAM); weights are rounded to the kind's type as well */
+                                         picks STREAM). (q - z) s is rounded to the kind's type, and q - z before that where z
+                                         is not a whole number up to 64 in magnitude: half a step of each weight, with the
+                                         result's rounding 1.3 times that one alone (root mean square). f16: a weight above
+                                         65504 is an infinity (scales above 4366 at q - z = 15), and one below 2^-14, as only
+                                         zero points with a fraction give, is off by up to 2^-25 */
 };
 typedef struct {
   int32_t kind;
@@ -668,11 +675,13 @@ typedef struct {
   int32_t lda, ldo;
   int32_t variant; /* IREE_B200_W4A16_EXPERTS_* */
 } iree_b200_w4a16_experts_params_t;
-/* prepare() picks the variant (TENSOR above 8 rows per expert, where its copies reach the operands) and writes what it needs
- * into the workspace: 128-byte aligned, the given size, not shared between dispatches in flight; for TENSOR this is a copy,
- * which a graph that is being recorded refuses (FAILED_PRECONDITION). run() dispatches and may be repeated, and recorded, while
- * operands stay in place; with other operands or sizes than prepare() saw, TENSOR computes nothing and
- * iree_b200_workspace_status reports INVALID_ARGUMENT. */
+/* prepare() picks the variant and writes what it needs into the workspace: 128-byte aligned, the given size, not shared between
+ * dispatches in flight; for TENSOR this is a copy, which a graph that is being recorded refuses (FAILED_PRECONDITION). AUTO goes
+ * by the room for rows, since the host does not know how many there are: TENSOR above 8 of params.rows per expert, where its
+ * copies reach the operands (and its tiles of 256 rows above 64 per expert, of 64 rows below). A rank that owns a part of the
+ * experts has room for all slots and uses its part: there, or where weights are not to be rounded, name the variant. run()
+ * dispatches and may be repeated, and recorded, while operands stay in place; with other operands or sizes than prepare() saw,
+ * TENSOR computes nothing and iree_b200_workspace_status reports INVALID_ARGUMENT. */
 size_t iree_b200_w4a16_experts_workspace_bytes(const iree_b200_w4a16_experts_params_t* params);
 iree_b200_status_t iree_b200_w4a16_experts_prepare(iree_b200_context_t* context,
                                                    const iree_b200_w4a16_experts_params_t* params, const void* a,

@@ -83,3 +83,23 @@ def test_weights_that_do_not_exist_are_not_formed(ctx, counts, K, group, kind, v
     for e in range(E):
         exact = a[off[e]:off[e + 1]] @ ((w.q[e] - 15) * s).T      # whole numbers up to 288, times one number of 11 bits
         assert (got[off[e]:off[e + 1]] == to_bits(exact, kind)).all()
+
+
+@pytest.mark.parametrize("variant", [ib.W4A16_EXPERTS_STREAM, ib.W4A16_EXPERTS_TENSOR])
+@pytest.mark.parametrize("zeros", [False, True])
+@pytest.mark.parametrize("step", [2.0 ** -14, 2.0 ** -18, 2.0 ** -24])
+def test_f16_scales_without_a_leading_digit(ctx, step, zeros, variant):
+    """Scales down to f16's smallest number, whole zero points: whole multiples of 2^-24, which 16 bits hold; the sums are whole
+    multiples of the scale too."""
+    rng = np.random.default_rng([int(-np.log2(step)), int(zeros)])
+    counts, N, K, group = [20, 70], 40, 256, 64
+    w = Weights(rng, F16, 2, N, K, group, zeros)
+    times = rng.integers(1, 4, w.scales.shape)
+    s = np.repeat(times * step, group, axis=-1)
+    w.scales = to_bits(times * step, F16)
+    q = w.q - np.repeat(to_f64(w.zeros, F16), group, axis=-1) if zeros else np.where(w.q >= 8, w.q - 16, w.q)
+    a = rng.integers(-2, 3, (sum(counts), K)).astype(np.float64)
+    got = run_experts(ctx, F16, counts, sum(counts), w, group, to_bits(a, F16), variant)
+    off = offsets_of(counts)
+    for e in range(2):
+        assert (to_f64(got[off[e]:off[e + 1]], F16) == to_f64(to_bits(a[off[e]:off[e + 1]] @ (q[e] * s[e]).T, F16), F16)).all()
