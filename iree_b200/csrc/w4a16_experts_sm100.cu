@@ -75,7 +75,7 @@ template <int AROWS>
 struct ExWalk {
   const int* first;  // tiles before each expert
   const int* row;    // rows before each expert
-  int tiles_n, e;
+  int e;
   __device__ ExTile at(int t) {
     while (first[e + 1] <= t) ++e;
     const int local = t - first[e], count = row[e + 1] - row[e];
@@ -243,7 +243,7 @@ __device__ void experts_body(const uint16_t* __restrict__ scales, const uint16_t
   const uint32_t tmem_base = *tmem_slot_ptr;
   const uint32_t tmem_a = tmem_base + AROWS;
   const int num_tiles = tile_first[experts];
-  ExWalk<AROWS> walk = {tile_first, row_first, tiles_n, 0};
+  ExWalk<AROWS> walk = {tile_first, row_first, 0};
 
   // The single-thread roles: the whole warp walks the loop and one elected thread issues, so that the operands of copies and
   // matrix instructions are values which the compiler knows to be uniform and need no move each from a thread's registers

@@ -13,9 +13,9 @@
 // cancels is at most 158 / 15 of the sum it leaves, 2^-20 of it in f32. In bf16 everything up to the result is kept 2^-15 times
 // its value, which costs nothing (sums of activations are formed that way, the result is multiplied once): activations reach
 // f32's largest numbers, and 128 of them times 143 would pass it where the scaled sum is a number again. What that takes from
-// the other end: sums below 2^-111 round in steps of 2^-149 of f32's subnormals, 2^-134 of the value. (f16 subnormals, q 2^-24 as stored, would spare the shifts; but the tensor core
-// aligns products by their exponent fields, and sums lost up to six more bits there.) The accumulator starts
-// at minus that offset times the sum of a.
+// the other end: sums below 2^-111 round in steps of 2^-149 of f32's subnormals, 2^-134 of the value. (f16 subnormals, q 2^-24 as
+// stored, would spare the shifts; but the tensor core aligns products by their exponent fields, and sums lost up to six more bits
+// there.) The accumulator starts at minus that offset times the sum of a.
 //
 // Work. The weight rows of all active experts (one, for a matrix-vector product) form one list; every CTA gets an equal
 // part of it, to the row, so that all SMs read the same number of bytes (tiles of 16 rows alone would leave the last round
@@ -147,11 +147,6 @@ __device__ __forceinline__ uint32_t stream_lds16(uint32_t addr) {
   asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(addr));
   return v;
 }
-__device__ __forceinline__ uint32_t and_xor(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(r) : "r"(a), "r"(b), "r"(c));  // (a & b) ^ c
-  return r;
-}
 // d = a b + c, c being (c0, c1) in both rows.
 template <bool BF16>
 __device__ __forceinline__ void mma_16816_first(float (&d)[4], float c0, float c1, uint32_t a0, uint32_t a1, uint32_t a2,
@@ -185,10 +180,7 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   } else {
-    asm volatile(
-        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    mma_m16n8k16(d, a0, a1, a2, a3, b0, b1);
   }
 }
 template <bool BF16>
@@ -546,10 +538,10 @@ __device__ void stream_body(const StreamArgs& p) {
               for (int i = 0; i < 2; ++i) {
                 const uint32_t w0 = i ? w.z : w.x, w1 = i ? w.w : w.y;
                 // nibbles (0, 4), (2, 6) and (1, 5), (3, 7) of either row
-                const uint32_t a0 = and_xor(BF16 ? w0 : w0 << 4, mask, under), a1 = and_xor(BF16 ? w1 : w1 << 4, mask, under);
-                const uint32_t a2 = and_xor(w0 >> (BF16 ? 8 : 4), mask, under), a3 = and_xor(w1 >> (BF16 ? 8 : 4), mask, under);
-                const uint32_t c0 = and_xor(BF16 ? w0 >> 4 : w0, mask, under), c1 = and_xor(BF16 ? w1 >> 4 : w1, mask, under);
-                const uint32_t c2 = and_xor(w0 >> (BF16 ? 12 : 8), mask, under), c3 = and_xor(w1 >> (BF16 ? 12 : 8), mask, under);
+                const uint32_t a0 = lop3_and_xor(BF16 ? w0 : w0 << 4, mask, under), a1 = lop3_and_xor(BF16 ? w1 : w1 << 4, mask, under);
+                const uint32_t a2 = lop3_and_xor(w0 >> (BF16 ? 8 : 4), mask, under), a3 = lop3_and_xor(w1 >> (BF16 ? 8 : 4), mask, under);
+                const uint32_t c0 = lop3_and_xor(BF16 ? w0 >> 4 : w0, mask, under), c1 = lop3_and_xor(BF16 ? w1 >> 4 : w1, mask, under);
+                const uint32_t c2 = lop3_and_xor(w0 >> (BF16 ? 12 : 8), mask, under), c3 = lop3_and_xor(w1 >> (BF16 ? 12 : 8), mask, under);
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
                   if (h == 0)
