@@ -240,6 +240,7 @@ class Context:
         in order with torch's work on their tensors, and memory that torch hands out again is not still in use here."""
         handle = getattr(stream, "cuda_stream", stream)
         check(library().iree_hal_b200_device_set_stream(self.device, C.c_void_p(None if handle is None else handle or 1)))
+        self._stream = stream  # lives as long as work is queued on it
 
     @property
     def launch_count(self) -> int:
