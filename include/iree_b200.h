@@ -619,7 +619,7 @@ typedef struct {
   int32_t slots;        /* experts per token, 1..256 */
   int32_t experts;      /* experts of this rank, 1..1024 */
   int32_t first_expert; /* id of its first one; a slot with an id outside [first_expert, first_expert + experts) is dropped */
-  int32_t width;        /* elements per row */
+  int32_t width;        /* elements per row, at most 2^31 - 4097 */
   int32_t token_pitch;  /* row pitch of x / out / dout / dx, in elements */
   int32_t row_pitch;    /* row pitch of rows / drows, in elements */
 } iree_b200_expert_rows_params_t;
@@ -660,10 +660,10 @@ enum {
   IREE_B200_W4A16_EXPERTS_STREAM = 1, /* reads an expert's weights for 8 or 16 rows at a time; any alignment; rounds only the
                                          result */
   IREE_B200_W4A16_EXPERTS_TENSOR = 2, /* tcgen05 tiles of 128 weight rows x up to 256 rows; a and out on 16-byte boundaries,
-                                         lda and ldo multiples of 8, experts * N < 2^31 (INVALID_ARGUMENT otherwise; AUTO then
-                                         picks STREAM). (q - z) s is rounded to the kind's type, and q - z before that where z
-                                         is not a whole number up to 64 in magnitude: half a step of each weight, with the
-                                         result's rounding 1.3 times that one alone (root mean square). f16: a weight above
+                                         lda and ldo multiples of 8, experts * N <= 2^31 - 257 (INVALID_ARGUMENT otherwise;
+                                         AUTO then picks STREAM). (q - z) s is rounded to the kind's type, and q - z before that
+                                         where z is not a whole number up to 64 in magnitude: half a step of each weight, with
+                                         the result's rounding 1.3 times that one alone (root mean square). f16: a weight above
                                          65504 is an infinity (scales above 4366 at q - z = 15), and one below 2^-14, as only
                                          zero points with a fraction give, is off by up to 2^-25 */
 };

@@ -216,7 +216,7 @@ extern "C" __global__ void __launch_bounds__(b200::kRouteThreads)
     for (int64_t i = kept + static_cast<int64_t>(blockIdx.x) * kRouteThreads + tid; i < all;
          i += static_cast<int64_t>(gridDim.x) * kRouteThreads)
       order[i] = -1;
-  const int d0 = blockIdx.y * part_width, d1 = min(width, d0 + part_width);
+  const int d0 = blockIdx.y * part_width, d1 = width - d0 < part_width ? width : d0 + part_width;
   const int tokens_at_once = max(1, kRouteRun / slots);
   for (int64_t t0 = t_lo; t0 < t_hi; t0 += tokens_at_once) {
     const int nt = static_cast<int>(min(static_cast<int64_t>(tokens_at_once), t_hi - t0));

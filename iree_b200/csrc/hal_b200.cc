@@ -1792,6 +1792,7 @@ constexpr uint32_t kRouteSmemBytes = (4 + 4 + 4 + 2 * 16) * 1024 + 4 * (1 + 512)
 constexpr int kMaxExperts = 1024;
 constexpr uint32_t kExpertsNoteMagic = 0x45585034u;
 constexpr int kMaxSlots = 256;
+constexpr int kMaxRowWidth = INT32_MAX - 4096;  // a strip of columns that starts inside a row ends inside 31 bits
 constexpr int kMaxStreamK = 1 << 20;  // the kernels divide K / 32 by group / 32 through a 32-bit reciprocal
 // Up to this many slots every CTA of the routing kernel counts all of them itself (one launch).
 constexpr int64_t kRouteSingleSlots = 8192;
@@ -2600,7 +2601,7 @@ static iree_b200_status_t encode_output_map(const void* device_ptr, uint32_t col
 // What the tensor-core kernel's TMA copies need.
 static bool experts_tensor_fits(const iree_b200_w4a16_experts_params_t* p, const void* a, const void* wq, const void* out) {
   return !misaligned(a, 16) && !misaligned(wq, 16) && !misaligned(out, 16) && p->lda % 8 == 0 && p->ldo % 8 == 0 &&
-         static_cast<int64_t>(p->experts) * p->N <= INT32_MAX;
+         static_cast<int64_t>(p->experts) * p->N <= INT32_MAX - 256;  // the last tile of 128 rows ends inside 31 bits
 }
 // Rows per expert above which the tensor-core kernels are the faster ones (11008 x 4096, 8 experts: 8 rows each 60 us streamed
 // against 66 us, 16 rows 88 against 67), and up to which their tiles of 64 rows are (64 rows 71 us, against 105 with 256).
@@ -2644,7 +2645,7 @@ iree_b200_status_t iree_b200_w4a16_experts_prepare(iree_b200_context_t* context,
     if (!a || !wq || !out) return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "operand pointer is NULL");
     if (!experts_tensor_fits(params, a, wq, out))
       return fail(IREE_B200_STATUS_INVALID_ARGUMENT,
-                  "the tensor-core kernel needs 16-byte aligned operands, pitches that are multiples of 8 and experts * N < 2^31");
+                  "the tensor-core kernel needs 16-byte aligned operands, pitches that are multiples of 8 and experts * N <= 2^31 - 257");
     if (!workspace || misaligned(workspace, 128))
       return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "workspace must be a 128-byte aligned device buffer");
   }
@@ -2687,7 +2688,7 @@ iree_b200_status_t iree_b200_w4a16_experts_run(iree_b200_context_t* context, con
       return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "offsets must be a 4-byte aligned device array");
     if (tensor && !experts_tensor_fits(params, a, wq, out))
       return fail(IREE_B200_STATUS_INVALID_ARGUMENT,
-                  "the tensor-core kernel needs 16-byte aligned operands, pitches that are multiples of 8 and experts * N < 2^31");
+                  "the tensor-core kernel needs 16-byte aligned operands, pitches that are multiples of 8 and experts * N <= 2^31 - 257");
     if (tensor && (!workspace || misaligned(workspace, 128)))
       return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "workspace must be a 128-byte aligned device buffer");
   }
@@ -2728,6 +2729,7 @@ static iree_b200_status_t rows_validate(const iree_b200_expert_rows_params_t* p)
     return fail(IREE_B200_STATUS_OUT_OF_RANGE, "1 to %d experts (got %d)", kMaxExperts, p->experts);
   if (static_cast<int64_t>(p->tokens) * p->slots > INT32_MAX)
     return fail(IREE_B200_STATUS_OUT_OF_RANGE, "%d tokens x %d slots do not fit 31 bits", p->tokens, p->slots);
+  if (p->width > kMaxRowWidth) return fail(IREE_B200_STATUS_OUT_OF_RANGE, "rows are at most %d wide (got %d)", kMaxRowWidth, p->width);
   if (p->token_pitch < p->width || p->row_pitch < p->width)
     return fail(IREE_B200_STATUS_INVALID_ARGUMENT, "row pitches %d and %d cannot hold %d elements", p->token_pitch, p->row_pitch,
                 p->width);
@@ -2781,9 +2783,10 @@ static void route_grid(const iree_b200_expert_rows_params_t* p, int sms, int* ru
   const int most = (p->width + 255) / 256;
   if (cut > most) cut = most;
   if (cut < 1) cut = 1;
-  *part_width = ((p->width + cut - 1) / cut + 63) & ~63;
+  const int64_t width = p->width;
+  *part_width = static_cast<int>(((width + cut - 1) / cut + 63) & ~63);
   if (*part_width < 64) *part_width = 64;
-  *parts = p->width ? (p->width + *part_width - 1) / *part_width : 1;
+  *parts = width ? static_cast<int>((width + *part_width - 1) / *part_width) : 1;
 }
 
 size_t iree_b200_expert_dispatch_workspace_bytes(const iree_b200_expert_rows_params_t* params) {
