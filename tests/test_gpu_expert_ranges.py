@@ -103,3 +103,22 @@ def test_f16_scales_without_a_leading_digit(ctx, step, zeros, variant):
     off = offsets_of(counts)
     for e in range(2):
         assert (to_f64(got[off[e]:off[e + 1]], F16) == to_f64(to_bits(a[off[e]:off[e + 1]] @ (q[e] * s[e]).T, F16), F16)).all()
+
+
+@pytest.mark.parametrize("variant", [ib.W4A16_EXPERTS_STREAM, ib.W4A16_EXPERTS_TENSOR])
+@pytest.mark.parametrize("kind", [F16, BF16])
+@pytest.mark.parametrize("counts", [[7, 30], [200, 101]])
+def test_what_is_not_finite_stays_in_its_row_and_column(ctx, counts, kind, variant):
+    rng = np.random.default_rng(19)
+    N, K, group, rows = 72, 320, 64, sum(counts)
+    w = Weights(rng, kind, 2, N, K, group, True)
+    a = to_bits(rng.standard_normal((rows, K)), kind)
+    clean = run_experts(ctx, kind, counts, rows, w, group, a, variant)
+    inf, nan = (0x7C00, 0x7E00) if kind == F16 else (0x7F80, 0x7FC0)
+    a[2, 7], a[counts[0] - 1, 100], a[rows - 1, K - 1] = inf, nan, inf
+    w.scales[0, 5, 1], w.zeros[1, 70, 4] = nan, nan
+    got = run_experts(ctx, kind, counts, rows, w, group, a, variant)
+    bad = np.zeros((rows, N), bool)
+    bad[[2, counts[0] - 1, rows - 1]] = True
+    bad[:counts[0], 5] = bad[counts[0]:, 70] = True
+    assert (got[~bad] == clean[~bad]).all() and not np.isfinite(to_f64(got[bad], kind)).any()
